@@ -63,9 +63,13 @@ int lv_abi_version(void);
  * [0, num_cache_blocks) reads block 0; a slot >= num_blocks * block_size is
  * not written) and raise a bit in a device-side error word:
  *   LV_DEVERR_BLOCK_ID  a block-table entry outside [0, num_cache_blocks)
- *                       (lv_paged_attention, lv_paged_attention_prefix)
+ *                       (lv_paged_attention, lv_paged_attention_prefix,
+ *                       lv_paged_attention_quant, lv_tree_attention,
+ *                       lv_tree_attention_quant)
  *   LV_DEVERR_SLOT      a slot_mapping entry >= num_blocks * block_size
- *                       (lv_kv_scatter, lv_qk_norm_rope_cache)
+ *                       (lv_kv_scatter, lv_qk_norm_rope_cache,
+ *                       lv_kv_scatter_quant, lv_qk_norm_rope_cache_quant;
+ *                       lv_kv_gather_quant, whose row is then zeros)
  * Negative slots are padding (skipped, no bit).
  * lv_device_errors waits for the current device (hipDeviceSynchronize), so
  * every kernel enqueued before the call has reported, then stores the bits
@@ -424,6 +428,149 @@ int lv_linear(const void* x_dev, int64_t x_stride_t, const void* weight_dev,
 int lv_linear_f32(const float* x_dev, int64_t x_stride_t, const float* weight_dev,
                   int64_t weight_stride_n, float* y_dev, int64_t y_stride_t, int64_t m, int64_t n,
                   int64_t k, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 8-bit paged K/V cache.  The reference has none: its cache holds the model's
+ * dtype (litevllm/cache/kv_cache.py:41-50).  A cached row -- the head_dim
+ * values x of one token and kv head -- is head_dim codes and one fp32 scale:
+ *   scale = fl32(max|x| / top),  code = nearest(fl32(x / scale))
+ *   value = code * scale
+ *   LV_INT8: codes are whole numbers in [-127, 127], top = 127
+ *   LV_E4M3: codes are OCP e4m3 values, top = 448
+ * rounded to nearest, ties to even.  A row of zeros has scale 0 and codes 0.
+ * A row with a value that is not finite has scale NaN and codes 0: all of it
+ * reads as NaN.  (A row whose largest magnitude is under about 2^-118 loses
+ * accuracy with its scale, a subnormal number.)
+ * Codes and scales lie anywhere a stride describes: element (block, token in
+ * block, head, dim) of the codes at block * stride_block + token *
+ * stride_token + head * stride_head + dim (code strides multiples of 16 and at
+ * least head_dim, codes 16-byte aligned), the scale of (block, token, head)
+ * likewise.  Keys and values share the strides.  Attention reads it fastest
+ * with each head's 16 rows of a block in one run (stride_token = head_dim,
+ * scale_stride_token = 1).
+ * ---------------------------------------------------------------------- */
+typedef enum lv_code {
+  LV_INT8 = 0,
+  LV_E4M3 = 1
+} lv_code;
+
+typedef struct lv_quant_cache {   /* in host memory, read during the call */
+  void* key_dev;                  /* codes, one byte each */
+  void* value_dev;
+  float* key_scale_dev;
+  float* value_scale_dev;
+  int64_t num_blocks;
+  int64_t stride_block, stride_token, stride_head;
+  int64_t scale_stride_block, scale_stride_token, scale_stride_head;
+  int32_t block_size, num_kv_heads, head_dim;
+  int32_t code;                   /* lv_code */
+} lv_quant_cache;
+
+/* lv_kv_scatter into an 8-bit cache: key/value rows of `dtype` (fp32, fp16,
+ * bf16) quantised at their slots.  Slots as in lv_kv_scatter; two tokens of
+ * one call at the same slot leave that row undefined (codes and scale may be
+ * of either).  head_dim 64, 128 or 256. */
+int lv_kv_scatter_quant(const void* key_dev, int64_t key_stride_t, const void* value_dev,
+                        int64_t value_stride_t, const lv_quant_cache* cache,
+                        const int64_t* slot_mapping_dev, int64_t num_tokens, lv_dtype dtype,
+                        void* stream);
+
+/* The rows at the given slots as values of `dtype` (fp32 products, rounded
+ * once): key/value [T, num_kv_heads, head_dim] with free token strides.
+ * Slots < 0 give rows of zeros, slots >= num_blocks * block_size too (and
+ * raise LV_DEVERR_SLOT). */
+int lv_kv_gather_quant(const lv_quant_cache* cache, const int64_t* slots_dev, int64_t num_tokens,
+                       void* key_dev, int64_t key_stride_t, void* value_dev,
+                       int64_t value_stride_t, lv_dtype dtype, void* stream);
+
+/* lv_qk_norm_rope_cache into an 8-bit cache (the same reference code).  The
+ * rows stay in fp32 from the projection's values to the query's one rounding
+ * and to the codes, where lv_qk_norm_rope_cache rounds every step to `dtype`;
+ * cos / sin and the norm weights are of `dtype`.  Any alignment (16-byte
+ * aligned rows, weights and cos / sin are faster). */
+int lv_qk_norm_rope_cache_quant(const void* qkv_dev, int64_t qkv_stride_t,
+                                const void* q_norm_weight_dev, const void* k_norm_weight_dev,
+                                const void* cos_dev, const void* sin_dev, int64_t max_position,
+                                const int64_t* positions_dev, const int64_t* slot_mapping_dev,
+                                void* q_out_dev, int64_t q_out_stride_t,
+                                const lv_quant_cache* cache, int64_t num_tokens,
+                                int32_t num_heads, float eps, lv_dtype dtype, void* stream);
+
+/* lv_paged_attention over an 8-bit cache: the same batch, the same rows
+ * (decodes first, then causal chunks at any offset), queries and outputs of
+ * `dtype`.  The softmax statistics and sums are fp32.  A row that sees no key
+ * (context length 0) is zeros.  Rows at or past cu_seqlens[num_seqs] are left
+ * as they were.  num_decodes tells which kernel serves a sequence, not what
+ * is computed: it may be 0.
+ * Supported: head_dim 64 or 128, block_size 16, num_heads a multiple of
+ * num_kv_heads (else LV_ERR_UNSUPPORTED).  workspace: at least
+ * lv_paged_attention_quant_workspace_size(...) bytes, 256-B aligned, contents
+ * need not be initialised, one per stream (and one per captured graph that
+ * may run beside another). */
+size_t lv_paged_attention_quant_workspace_size(int32_t num_seqs, int32_t num_decodes,
+                                               int64_t num_tokens, int32_t max_query_len,
+                                               int32_t num_heads, int32_t num_kv_heads,
+                                               int32_t head_dim, int32_t max_blocks,
+                                               lv_dtype dtype);
+
+int lv_paged_attention_quant(const void* query_dev, int64_t q_stride_t,
+                             const lv_quant_cache* cache, const int32_t* block_tables_dev,
+                             int32_t max_blocks, const int32_t* cu_seqlens_dev,
+                             const int32_t* context_lens_dev, int32_t num_seqs,
+                             int32_t num_decodes, int64_t num_tokens, int32_t max_query_len,
+                             int32_t num_heads, float scale, void* out_dev, int64_t out_stride_t,
+                             void* workspace_dev, size_t workspace_bytes, lv_dtype dtype,
+                             void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention for trees of drafted tokens (speculative decoding).  The
+ * reference decodes one token per sequence and step (layers/attention.py:
+ * 91-139).  Here sequence i feeds n_i = cu_seqlens[i + 1] - cu_seqlens[i]
+ * drafted tokens whose K/V are already in the cache behind its committed
+ * tokens, in row order: context_lens[i] counts both.  Row j sees every
+ * committed key (position < context_lens[i] - n_i) and the drafted key t
+ * (position context_lens[i] - n_i + t) where bit t of its mask row is set:
+ * bit t % 64 of tree_mask[row][t / 64].  A row sees itself only if its own bit
+ * is set; a row that sees nothing is zeros.  A drafted key that a row does not
+ * see has no influence on it, whatever it holds.
+ * tree_mask: uint64 [num_tokens, mask_words], mask_words * 64 >= max_query_len.
+ * Caches of lv_tree_attention: contiguous, of `dtype`, as in
+ * lv_paged_attention.  Other arguments, limits and the workspace as in
+ * lv_paged_attention_quant (size from lv_tree_attention_workspace_size for
+ * both entries). */
+size_t lv_tree_attention_workspace_size(int32_t num_seqs, int64_t num_tokens,
+                                        int32_t max_query_len, int32_t num_heads,
+                                        int32_t num_kv_heads, int32_t head_dim,
+                                        int32_t max_blocks, lv_dtype dtype);
+
+int lv_tree_attention(const void* query_dev, int64_t q_stride_t, const void* key_cache_dev,
+                      const void* value_cache_dev, int64_t num_cache_blocks,
+                      const int32_t* block_tables_dev, int32_t max_blocks,
+                      const int32_t* cu_seqlens_dev, const int32_t* context_lens_dev,
+                      const uint64_t* tree_mask_dev, int32_t mask_words, int32_t num_seqs,
+                      int64_t num_tokens, int32_t max_query_len, int32_t num_heads,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
+                      void* out_dev, int64_t out_stride_t, void* workspace_dev,
+                      size_t workspace_bytes, lv_dtype dtype, void* stream);
+
+int lv_tree_attention_quant(const void* query_dev, int64_t q_stride_t,
+                            const lv_quant_cache* cache, const int32_t* block_tables_dev,
+                            int32_t max_blocks, const int32_t* cu_seqlens_dev,
+                            const int32_t* context_lens_dev, const uint64_t* tree_mask_dev,
+                            int32_t mask_words, int32_t num_seqs, int64_t num_tokens,
+                            int32_t max_query_len, int32_t num_heads, float scale, void* out_dev,
+                            int64_t out_stride_t, void* workspace_dev, size_t workspace_bytes,
+                            lv_dtype dtype, void* stream);
+
+/* Mask rows of trees given by parents: parents [num_tokens] holds for each
+ * drafted token the index of its parent among its sequence's drafted tokens,
+ * or a negative number for a token that follows the committed ones.  A parent
+ * comes before its children: an index that does not (>= the token's own) is
+ * taken as no parent.  Row j gets the bits of j, its parent, that one's
+ * parent, ...; rows of no sequence are left as they were.  mask_words 1 to 16;
+ * tokens past 64 * mask_words of a sequence have no bit. */
+int lv_tree_mask(const int32_t* parents_dev, const int32_t* cu_seqlens_dev, int32_t num_seqs,
+                 int64_t num_tokens, uint64_t* tree_mask_dev, int32_t mask_words, void* stream);
 
 #ifdef __cplusplus
 }

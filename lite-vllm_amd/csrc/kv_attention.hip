@@ -1,0 +1,451 @@
+// Attention over the 8-bit paged cache, and attention for trees of drafted
+// tokens over either cache.
+//
+// Query rows of a sequence follow its committed tokens; row j of n sees the
+// keys a mask gives it: all positions up to its own (causal), or the
+// committed ones and its ancestors among the drafted (tree).  For the cached
+// row (codes c, scale s) of a key, score and output are
+//   x_t = scale * s_t * (q . c_t),   o = sum_t w_t s'_t c'_t / sum_t w_t,
+//   w_t = exp(x_t - max)
+// with the codes taken as they are and the scales applied to fp32 values.
+#include <type_traits>
+
+#include "lv_common.h"
+#include "lv_quant.h"
+
+namespace lv {
+
+// A paged cache of element or code type; strides in elements.
+struct KvView {
+  const void* kv[2];
+  const float* scale[2];         // 8-bit caches only
+  int64_t blk, tok, head;
+  int64_t sblk, stok, shead;
+  int64_t num_blocks;
+};
+
+struct Batch {
+  const int32_t* block_tables; int max_blocks;
+  const int32_t* cu; const int32_t* ctx;
+  const uint64_t* mask; int mask_words;      // trees only
+  int num_seqs; int num_tokens;
+};
+
+struct Rows {
+  const void* q; int64_t q_stride;
+  void* out; int64_t out_stride;
+  int num_heads, num_kv_heads;
+  float scale_log2;
+};
+
+constexpr int kBs = 16;
+constexpr float kNegBig = -1.0e30f;
+
+template <typename C> struct cached {          // 8-bit codes
+  static constexpr bool kCodes = true;
+  static constexpr int kBytes = 1;
+  static constexpr int kPer16B = 16;
+  __device__ __forceinline__ static void unpack(const uint4& v, float* out) {
+    code<C>::unpack4(v.x, out);
+    code<C>::unpack4(v.y, out + 4);
+    code<C>::unpack4(v.z, out + 8);
+    code<C>::unpack4(v.w, out + 12);
+  }
+};
+template <typename T> struct cached_elem : elem<T> { static constexpr bool kCodes = false; };
+template <> struct cached<float> : cached_elem<float> {};
+template <> struct cached<f16> : cached_elem<f16> {};
+template <> struct cached<bf16> : cached_elem<bf16> {};
+
+// A sequence's query rows [q0, q0 + n) and its keys [0, ctx), clamped to the
+// batch's tensors.
+struct Seq { int q0, n, ctx; };
+__device__ __forceinline__ Seq sequence(const Batch& b, int i) {
+  Seq s;
+  s.q0 = b.cu ? b.cu[i] : i;
+  const int q1 = b.cu ? b.cu[i + 1] : i + 1;
+  s.q0 = min(max(s.q0, 0), b.num_tokens);
+  s.n = min(max(q1 - s.q0, 0), b.num_tokens - s.q0);
+  s.ctx = min(max(b.ctx[i], 0), b.max_blocks * kBs);
+  return s;
+}
+
+__device__ __forceinline__ int physical_block(const Batch& b, int64_t num_blocks, int seq,
+                                              int blk) {
+  const int id = b.block_tables[(int64_t)seq * b.max_blocks + blk];
+  if (id >= 0 && id < num_blocks) return id;
+  report_device_error(LV_DEVERR_BLOCK_ID);     // clamped and reported
+  return 0;
+}
+
+// One workgroup of 4 wavefronts per (query row, head).  A lane takes one key
+// of 64 for the scores (its whole row, against the query in LDS), then one or
+// two dims for the output (every key's weight broadcast by readlane), so no
+// row of the cache is ever spread and summed over lanes.  Right for every
+// type and mask, and the form that the others are held to: it reads the cache
+// once for every query row and head.
+template <typename T, typename C, int D, bool TREE>
+__global__ __launch_bounds__(256) void attn_row_kernel(Batch b, KvView c, Rows r) {
+  using E = cached<C>;
+  constexpr int P = E::kPer16B, DPL = D / 64;
+  __shared__ float s_q[D];
+  __shared__ float s_o[4][D];
+  __shared__ float s_ml[4][2];
+  const int row = blockIdx.x, head = blockIdx.y;
+  int seq = row;
+  if (b.cu) {
+    int lo = 0, hi = b.num_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (b.cu[mid] <= row) lo = mid; else hi = mid - 1;
+    }
+    seq = lo;
+  }
+  const Seq s = sequence(b, seq);
+  const int j = row - s.q0;
+  if (j < 0 || j >= s.n) return;
+  const int kvh = head / (r.num_heads / r.num_kv_heads);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const T* qp = (const T*)r.q + (int64_t)row * r.q_stride + (int64_t)head * D;
+  for (int d = threadIdx.x; d < D; d += 256) s_q[d] = elem<T>::load(qp + d) * r.scale_log2;
+  __syncthreads();
+  const char* kb = (const char*)c.kv[0] + (int64_t)kvh * c.head * E::kBytes;
+  const char* vb = (const char*)c.kv[1] + (int64_t)kvh * c.head * E::kBytes;
+  const int committed = s.ctx - s.n;
+  const int end = TREE ? s.ctx : min(s.ctx, committed + j + 1);
+  float m = kNegBig, l = 0.0f, o[DPL] = {};
+  for (int k0 = wave * 64; k0 < end; k0 += 256) {
+    const int key = k0 + lane;
+    bool sees = key < end;
+    if (TREE && sees && key >= committed) {
+      const int t = key - committed;
+      sees = (b.mask[(int64_t)row * b.mask_words + (t >> 6)] >> (t & 63)) & 1;
+    }
+    const int kc = min(key, end - 1);
+    const int64_t phys = physical_block(b, c.num_blocks, seq, kc / kBs);
+    const int off = kc % kBs;
+    const char* kp = kb + (phys * c.blk + off * c.tok) * E::kBytes;
+    float x = 0.0f;
+    for (int d = 0; d < D; d += P) {
+      float kf[P];
+      E::unpack(load16(kp + d * E::kBytes), kf);
+#pragma unroll
+      for (int i = 0; i < P; ++i) x = fmaf(s_q[d + i], kf[i], x);
+    }
+    float vs = 1.0f;
+    if constexpr (E::kCodes) {
+      const int64_t at = phys * c.sblk + off * c.stok + kvh * c.shead;
+      x *= c.scale[0][at];
+      vs = c.scale[1][at];
+    }
+    const float mx = fmaxf(m, group_max<64>(sees ? x : kNegBig));
+    const float alpha = fast_exp2(m - mx);
+    m = mx;
+    const float p = sees ? fast_exp2(x - m) : 0.0f;
+    l = l * alpha + p;
+    const float w = p * vs;
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) o[i] *= alpha;
+    uint64_t seen = __ballot(sees);
+    const int64_t vat = (phys * c.blk + off * c.tok) * E::kBytes;
+    while (seen) {       // (a key that is not seen is not read: it may hold anything)
+      const int k = __builtin_ctzll(seen);
+      seen &= seen - 1;
+      const float wk = __shfl(w, k);
+      const char* vp = vb + __shfl(vat, k);
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) {
+        const int d = lane + 64 * i;
+        float v;
+        if constexpr (E::kCodes) {
+          float four[4];
+          code<C>::unpack4(*(const uint8_t*)(vp + d), four);
+          v = four[0];
+        } else {
+          v = elem<C>::load((const C*)vp + d);
+        }
+        o[i] = fmaf(wk, v, o[i]);
+      }
+    }
+  }
+  l = group_sum<64>(l);
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) s_o[wave][lane + 64 * i] = o[i];
+  if (lane == 0) { s_ml[wave][0] = m; s_ml[wave][1] = l; }
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += 256) {
+    float mx = kNegBig, sum = 0.0f, acc = 0.0f;
+    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_ml[w][0]);
+    for (int w = 0; w < 4; ++w) {
+      const float f = fast_exp2(s_ml[w][0] - mx);
+      sum = fmaf(s_ml[w][1], f, sum);
+      acc = fmaf(s_o[w][d], f, acc);
+    }
+    elem<T>::store((T*)r.out + (int64_t)row * r.out_stride + (int64_t)head * D + d,
+                   sum != 0.0f ? acc / sum : 0.0f);
+  }
+}
+
+// Ancestor bits: thread per drafted token walks up its parents, whose indices
+// fall, so that every walk ends.
+__global__ __launch_bounds__(256) void tree_mask_kernel(const int32_t* __restrict__ parents,
+                                                        const int32_t* __restrict__ cu,
+                                                        int num_seqs, int num_tokens,
+                                                        uint64_t* __restrict__ mask, int words) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= num_tokens) return;
+  int lo = 0, hi = num_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= row) lo = mid; else hi = mid - 1;
+  }
+  const int q0 = cu[lo];
+  if (q0 < 0 || row < q0 || row >= cu[lo + 1]) return;
+  uint64_t* out = mask + (int64_t)row * words;
+  int at = row - q0;
+  for (int w = words - 1; w >= 0; --w) {     // the walk meets the words from the last down
+    uint64_t bits = 0;
+    while (at >= 64 * w) {
+      if (at < 64 * (w + 1)) bits |= 1ull << (at & 63);
+      const int up = parents[q0 + at];
+      at = up < at ? up : -1;
+      if (at < 0) break;
+    }
+    out[w] = bits;
+  }
+}
+
+LV_ERROR_WORD_READER(read_errors_tree)
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+namespace {
+
+struct Call {
+  Batch b; KvView c; Rows r;
+  int d; lv_dtype dtype; int code;     // code: lv_code, or -1 for a cache of dtype
+  bool tree;
+  hipStream_t stream;
+};
+
+template <typename T, typename C, int D>
+int launch_rows(const Call& a) {
+  const dim3 grid((unsigned)a.b.num_tokens, (unsigned)a.r.num_heads);
+  if (a.tree) attn_row_kernel<T, C, D, true><<<grid, 256, 0, a.stream>>>(a.b, a.c, a.r);
+  else attn_row_kernel<T, C, D, false><<<grid, 256, 0, a.stream>>>(a.b, a.c, a.r);
+  return check_launch("attn_row_kernel");
+}
+
+template <typename T, typename C>
+int launch_d(const Call& a) {
+  return a.d == 64 ? launch_rows<T, C, 64>(a) : launch_rows<T, C, 128>(a);
+}
+
+template <typename T>
+int launch_c(const Call& a) {
+  if (a.code == LV_INT8) return launch_d<T, int8_code>(a);
+  if (a.code == LV_E4M3) return launch_d<T, e4m3_code>(a);
+  return launch_d<T, T>(a);
+}
+
+int launch(const Call& a) {
+  if (a.dtype == LV_F32) return launch_c<float>(a);
+  if (a.dtype == LV_F16) return launch_c<f16>(a);
+  return launch_c<bf16>(a);
+}
+
+size_t workspace_size(int64_t num_tokens, int max_query_len, int num_heads, int num_kv_heads,
+                      int head_dim, int max_blocks) {
+  return 0;
+}
+
+// The checks common to the attention entries; fills `a` but for the cache.
+int check_call(const char* who, Call& a, const void* query, int64_t q_stride,
+               const int32_t* tables, int max_blocks, const int32_t* cu, const int32_t* ctx,
+               int num_seqs, int64_t num_tokens, int max_query_len, int num_heads,
+               int num_kv_heads, int head_dim, int block_size, float scale, void* out,
+               int64_t out_stride, const void* ws, size_t ws_bytes, lv_dtype dtype) {
+  LV_REQUIRE(dtype == LV_F32 || dtype == LV_F16 || dtype == LV_BF16, "%s: bad dtype", who);
+  LV_REQUIRE(num_seqs >= 0 && num_tokens >= 0 && max_blocks >= 0 && max_query_len >= 0,
+             "%s: negative size", who);
+  LV_REQUIRE(num_tokens < (1ll << 31), "%s: num_tokens does not fit in 32 bits", who);
+  LV_REQUIRE(max_blocks < (1 << 27), "%s: max_blocks * 16 does not fit in 32 bits", who);
+  LV_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0,
+             "%s: num_heads must be a multiple of num_kv_heads", who);
+  if ((head_dim != 64 && head_dim != 128) || block_size != kBs || num_heads > 65535) {
+    set_error("%s: head_dim %d, block_size %d, %d heads (head_dim 64 or 128, block_size 16 and "
+              "up to 65535 heads are supported)", who, head_dim, block_size, num_heads);
+    return LV_ERR_UNSUPPORTED;
+  }
+  if (num_seqs == 0 || num_tokens == 0) return LV_OK;
+  LV_REQUIRE(query && out && ctx && (tables || max_blocks == 0), "%s: null pointer", who);
+  LV_REQUIRE(cu || num_tokens == num_seqs, "%s: without cu_seqlens every sequence has one row",
+             who);
+  const int64_t row = (int64_t)num_heads * head_dim;
+  LV_REQUIRE((q_stride >= row && out_stride >= row) || num_tokens == 1,
+             "%s: token stride smaller than num_heads*head_dim", who);
+  const size_t es = dtype_size(dtype);
+  LV_REQUIRE(aligned16(query) && aligned16(out) && (q_stride * es) % 16 == 0 &&
+                 (out_stride * es) % 16 == 0,
+             "%s: query and out rows must be 16-byte aligned", who);
+  a.b.block_tables = tables; a.b.max_blocks = max_blocks;
+  a.b.cu = cu; a.b.ctx = ctx;
+  a.b.num_seqs = num_seqs; a.b.num_tokens = (int)num_tokens;
+  a.r.q = query; a.r.q_stride = q_stride; a.r.out = out; a.r.out_stride = out_stride;
+  a.r.num_heads = num_heads; a.r.num_kv_heads = num_kv_heads;
+  a.r.scale_log2 = scale * 1.4426950408889634f;
+  a.d = head_dim; a.dtype = dtype;
+  const size_t need = workspace_size(num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
+                                     max_blocks);
+  if (need > 0 && (!ws || ((uintptr_t)ws & 255) != 0 || ws_bytes < need)) {
+    set_error("%s: workspace of %zu bytes (256-byte aligned) needed, got %zu", who, need,
+              ws ? ws_bytes : (size_t)0);
+    return LV_ERR_WORKSPACE;
+  }
+  return LV_OK;
+}
+
+void use_cache(Call& a, const lv_quant_cache* c) {
+  a.c = KvView{{c->key_dev, c->value_dev}, {c->key_scale_dev, c->value_scale_dev},
+               c->stride_block, c->stride_token, c->stride_head,
+               c->scale_stride_block, c->scale_stride_token, c->scale_stride_head, c->num_blocks};
+  a.code = c->code;
+}
+
+int check_mask(const char* who, Call& a, const uint64_t* mask, int words, int max_query_len,
+               int64_t num_tokens) {
+  LV_REQUIRE(words >= 1 && (int64_t)words * 64 >= max_query_len,
+             "%s: mask_words * 64 must be at least max_query_len", who);
+  LV_REQUIRE((mask && ((uintptr_t)mask & 7) == 0) || num_tokens == 0,
+             "%s: null or unaligned tree_mask", who);
+  a.b.mask = mask;
+  a.b.mask_words = words;
+  a.tree = true;
+  return LV_OK;
+}
+
+}  // namespace
+}  // namespace lv
+
+extern "C" size_t lv_paged_attention_quant_workspace_size(int32_t num_seqs, int32_t num_decodes,
+                                                          int64_t num_tokens,
+                                                          int32_t max_query_len,
+                                                          int32_t num_heads,
+                                                          int32_t num_kv_heads, int32_t head_dim,
+                                                          int32_t max_blocks, lv_dtype dtype) {
+  return lv::workspace_size(num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
+                            max_blocks);
+}
+
+extern "C" size_t lv_tree_attention_workspace_size(int32_t num_seqs, int64_t num_tokens,
+                                                   int32_t max_query_len, int32_t num_heads,
+                                                   int32_t num_kv_heads, int32_t head_dim,
+                                                   int32_t max_blocks, lv_dtype dtype) {
+  return lv::workspace_size(num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
+                            max_blocks);
+}
+
+extern "C" int lv_paged_attention_quant(
+    const void* query_dev, int64_t q_stride_t, const lv_quant_cache* cache,
+    const int32_t* block_tables_dev, int32_t max_blocks, const int32_t* cu_seqlens_dev,
+    const int32_t* context_lens_dev, int32_t num_seqs, int32_t num_decodes, int64_t num_tokens,
+    int32_t max_query_len, int32_t num_heads, float scale, void* out_dev, int64_t out_stride_t,
+    void* workspace_dev, size_t workspace_bytes, lv_dtype dtype, void* stream) {
+  using namespace lv;
+  constexpr const char* who = "lv_paged_attention_quant";
+  clear_error();
+  if (const int rc = check_quant_cache(who, cache); rc != LV_OK) return rc;
+  LV_REQUIRE(num_decodes >= 0 && num_decodes <= num_seqs && num_decodes <= num_tokens,
+             "%s: num_decodes %d outside [0, num_seqs]", who, num_decodes);
+  Call a{};
+  if (const int rc = check_call(who, a, query_dev, q_stride_t, block_tables_dev, max_blocks,
+                                cu_seqlens_dev, context_lens_dev, num_seqs, num_tokens,
+                                max_query_len, num_heads, cache->num_kv_heads, cache->head_dim,
+                                cache->block_size, scale, out_dev, out_stride_t, workspace_dev,
+                                workspace_bytes, dtype);
+      rc != LV_OK || num_seqs == 0 || num_tokens == 0)
+    return rc;
+  use_cache(a, cache);
+  a.stream = (hipStream_t)stream;
+  return launch(a);
+}
+
+extern "C" int lv_tree_attention(
+    const void* query_dev, int64_t q_stride_t, const void* key_cache_dev,
+    const void* value_cache_dev, int64_t num_cache_blocks, const int32_t* block_tables_dev,
+    int32_t max_blocks, const int32_t* cu_seqlens_dev, const int32_t* context_lens_dev,
+    const uint64_t* tree_mask_dev, int32_t mask_words, int32_t num_seqs, int64_t num_tokens,
+    int32_t max_query_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t block_size, float scale, void* out_dev, int64_t out_stride_t, void* workspace_dev,
+    size_t workspace_bytes, lv_dtype dtype, void* stream) {
+  using namespace lv;
+  constexpr const char* who = "lv_tree_attention";
+  clear_error();
+  Call a{};
+  if (const int rc = check_mask(who, a, tree_mask_dev, mask_words, max_query_len, num_tokens);
+      rc != LV_OK)
+    return rc;
+  LV_REQUIRE(num_cache_blocks > 0, "%s: bad cache geometry", who);
+  if (const int rc = check_call(who, a, query_dev, q_stride_t, block_tables_dev, max_blocks,
+                                cu_seqlens_dev, context_lens_dev, num_seqs, num_tokens,
+                                max_query_len, num_heads, num_kv_heads, head_dim, block_size,
+                                scale, out_dev, out_stride_t, workspace_dev, workspace_bytes,
+                                dtype);
+      rc != LV_OK || num_seqs == 0 || num_tokens == 0)
+    return rc;
+  LV_REQUIRE(cu_seqlens_dev, "%s: null cu_seqlens", who);
+  LV_REQUIRE(key_cache_dev && value_cache_dev && aligned16(key_cache_dev) &&
+                 aligned16(value_cache_dev),
+             "%s: null or unaligned cache", who);
+  const int64_t tok = (int64_t)num_kv_heads * head_dim;
+  a.c = KvView{{key_cache_dev, value_cache_dev}, {nullptr, nullptr}, kBs * tok, tok, head_dim,
+               0, 0, 0, num_cache_blocks};
+  a.code = -1;
+  a.stream = (hipStream_t)stream;
+  return launch(a);
+}
+
+extern "C" int lv_tree_attention_quant(
+    const void* query_dev, int64_t q_stride_t, const lv_quant_cache* cache,
+    const int32_t* block_tables_dev, int32_t max_blocks, const int32_t* cu_seqlens_dev,
+    const int32_t* context_lens_dev, const uint64_t* tree_mask_dev, int32_t mask_words,
+    int32_t num_seqs, int64_t num_tokens, int32_t max_query_len, int32_t num_heads, float scale,
+    void* out_dev, int64_t out_stride_t, void* workspace_dev, size_t workspace_bytes,
+    lv_dtype dtype, void* stream) {
+  using namespace lv;
+  constexpr const char* who = "lv_tree_attention_quant";
+  clear_error();
+  if (const int rc = check_quant_cache(who, cache); rc != LV_OK) return rc;
+  Call a{};
+  if (const int rc = check_mask(who, a, tree_mask_dev, mask_words, max_query_len, num_tokens);
+      rc != LV_OK)
+    return rc;
+  if (const int rc = check_call(who, a, query_dev, q_stride_t, block_tables_dev, max_blocks,
+                                cu_seqlens_dev, context_lens_dev, num_seqs, num_tokens,
+                                max_query_len, num_heads, cache->num_kv_heads, cache->head_dim,
+                                cache->block_size, scale, out_dev, out_stride_t, workspace_dev,
+                                workspace_bytes, dtype);
+      rc != LV_OK || num_seqs == 0 || num_tokens == 0)
+    return rc;
+  LV_REQUIRE(cu_seqlens_dev, "%s: null cu_seqlens", who);
+  use_cache(a, cache);
+  a.stream = (hipStream_t)stream;
+  return launch(a);
+}
+
+extern "C" int lv_tree_mask(const int32_t* parents_dev, const int32_t* cu_seqlens_dev,
+                            int32_t num_seqs, int64_t num_tokens, uint64_t* tree_mask_dev,
+                            int32_t mask_words, void* stream) {
+  using namespace lv;
+  clear_error();
+  LV_REQUIRE(num_seqs >= 0 && num_tokens >= 0 && num_tokens < (1ll << 31),
+             "lv_tree_mask: bad sizes");
+  LV_REQUIRE(mask_words >= 1 && mask_words <= 16, "lv_tree_mask: mask_words must be 1 to 16");
+  if (num_seqs == 0 || num_tokens == 0) return LV_OK;
+  LV_REQUIRE(parents_dev && cu_seqlens_dev && tree_mask_dev && ((uintptr_t)tree_mask_dev & 7) == 0,
+             "lv_tree_mask: null or unaligned pointer");
+  tree_mask_kernel<<<(unsigned)((num_tokens + 255) / 256), 256, 0, (hipStream_t)stream>>>(
+      parents_dev, cu_seqlens_dev, num_seqs, (int)num_tokens, tree_mask_dev, mask_words);
+  return check_launch("lv_tree_mask");
+}

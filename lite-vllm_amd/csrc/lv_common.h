@@ -213,6 +213,11 @@ __device__ __forceinline__ void report_device_error(uint32_t bit) {
 int read_errors_scatter(uint32_t* bits, bool clear);
 int read_errors_attention(uint32_t* bits, bool clear);
 int read_errors_fused(uint32_t* bits, bool clear);
+int read_errors_quant(uint32_t* bits, bool clear);
+int read_errors_tree(uint32_t* bits, bool clear);
+
+// Checks a cache description on the host (kv_quant.hip).
+int check_quant_cache(const char* who, const lv_quant_cache* cache);
 
 #define LV_ERROR_WORD_READER(NAME)                                                        \
   int NAME(uint32_t* bits, bool clear) {                                                   \

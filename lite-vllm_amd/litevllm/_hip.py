@@ -17,6 +17,7 @@ LIB_NAME = "liblitevllm_hip.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 
 LV_F32, LV_F16, LV_BF16 = 0, 1, 2
+LV_INT8, LV_E4M3 = 0, 1
 LV_ACT_NONE, LV_ACT_SILU_MUL = 0, 1
 ABI_VERSION = 7
 LV_ERR_DEVICE_INDEX = -5
@@ -25,6 +26,17 @@ LV_DEVERR_BLOCK_ID, LV_DEVERR_SLOT = 1, 2
 # Every symbol the header declares, with (restype, argtypes).
 _c_i32, _c_i64, _c_f32, _c_p, _c_sz = (
     ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t)
+
+class QuantCache(ctypes.Structure):
+    """lv_quant_cache (include/litevllm_hip.h)."""
+    _fields_ = [(n, _c_p) for n in ("key", "value", "key_scale", "value_scale")] + \
+        [(n, _c_i64) for n in ("num_blocks", "stride_block", "stride_token", "stride_head",
+                               "scale_stride_block", "scale_stride_token",
+                               "scale_stride_head")] + \
+        [(n, _c_i32) for n in ("block_size", "num_kv_heads", "head_dim", "code")]
+
+
+_c_cache = ctypes.POINTER(QuantCache)
 
 SIGNATURES: dict[str, tuple] = {
     "lv_last_error": (ctypes.c_char_p, []),
@@ -130,6 +142,65 @@ SIGNATURES: dict[str, tuple] = {
         _c_p, _c_i64, _c_p, _c_i64,    # x, x_stride, weight, weight_stride
         _c_p, _c_i64,                  # y, y_stride
         _c_i64, _c_i64, _c_i64, _c_p,  # m, n, k, stream
+    ]),
+    "lv_kv_scatter_quant": (ctypes.c_int, [
+        _c_p, _c_i64, _c_p, _c_i64,    # key, key_stride_t, value, value_stride_t
+        _c_cache, _c_p, _c_i64,        # cache, slot_mapping, num_tokens
+        ctypes.c_int, _c_p,            # dtype, stream
+    ]),
+    "lv_kv_gather_quant": (ctypes.c_int, [
+        _c_cache, _c_p, _c_i64,        # cache, slots, num_tokens
+        _c_p, _c_i64, _c_p, _c_i64,    # key, key_stride_t, value, value_stride_t
+        ctypes.c_int, _c_p,            # dtype, stream
+    ]),
+    "lv_qk_norm_rope_cache_quant": (ctypes.c_int, [
+        _c_p, _c_i64, _c_p, _c_p,      # qkv, qkv_stride, q_norm_w, k_norm_w
+        _c_p, _c_p, _c_i64,            # cos, sin, max_position
+        _c_p, _c_p, _c_p, _c_i64,      # positions, slot_mapping, q_out, q_out_stride
+        _c_cache, _c_i64, _c_i32,      # cache, num_tokens, num_heads
+        ctypes.c_float, ctypes.c_int, _c_p,  # eps, dtype, stream
+    ]),
+    "lv_paged_attention_quant_workspace_size": (_c_sz, [
+        _c_i32, _c_i32, _c_i64, _c_i32,  # num_seqs, num_decodes, num_tokens, max_query_len
+        _c_i32, _c_i32, _c_i32, _c_i32,  # num_heads, num_kv_heads, head_dim, max_blocks
+        ctypes.c_int,                  # dtype
+    ]),
+    "lv_paged_attention_quant": (ctypes.c_int, [
+        _c_p, _c_i64, _c_cache,        # query, q_stride_t, cache
+        _c_p, _c_i32, _c_p, _c_p,      # block_tables, max_blocks, cu_seqlens, context_lens
+        _c_i32, _c_i32, _c_i64, _c_i32,  # num_seqs, num_decodes, num_tokens, max_query_len
+        _c_i32, _c_f32, _c_p, _c_i64,  # num_heads, scale, out, out_stride_t
+        _c_p, _c_sz,                   # workspace, workspace_bytes
+        ctypes.c_int, _c_p,            # dtype, stream
+    ]),
+    "lv_tree_attention_workspace_size": (_c_sz, [
+        _c_i32, _c_i64, _c_i32,        # num_seqs, num_tokens, max_query_len
+        _c_i32, _c_i32, _c_i32, _c_i32,  # num_heads, num_kv_heads, head_dim, max_blocks
+        ctypes.c_int,                  # dtype
+    ]),
+    "lv_tree_attention": (ctypes.c_int, [
+        _c_p, _c_i64,                  # query, q_stride_t
+        _c_p, _c_p, _c_i64,            # key_cache, value_cache, num_cache_blocks
+        _c_p, _c_i32, _c_p, _c_p,      # block_tables, max_blocks, cu_seqlens, context_lens
+        _c_p, _c_i32,                  # tree_mask, mask_words
+        _c_i32, _c_i64, _c_i32,        # num_seqs, num_tokens, max_query_len
+        _c_i32, _c_i32, _c_i32,        # num_heads, num_kv_heads, head_dim
+        _c_i32, _c_f32, _c_p, _c_i64,  # block_size, scale, out, out_stride_t
+        _c_p, _c_sz,                   # workspace, workspace_bytes
+        ctypes.c_int, _c_p,            # dtype, stream
+    ]),
+    "lv_tree_attention_quant": (ctypes.c_int, [
+        _c_p, _c_i64, _c_cache,        # query, q_stride_t, cache
+        _c_p, _c_i32, _c_p, _c_p,      # block_tables, max_blocks, cu_seqlens, context_lens
+        _c_p, _c_i32,                  # tree_mask, mask_words
+        _c_i32, _c_i64, _c_i32,        # num_seqs, num_tokens, max_query_len
+        _c_i32, _c_f32, _c_p, _c_i64,  # num_heads, scale, out, out_stride_t
+        _c_p, _c_sz,                   # workspace, workspace_bytes
+        ctypes.c_int, _c_p,            # dtype, stream
+    ]),
+    "lv_tree_mask": (ctypes.c_int, [
+        _c_p, _c_p, _c_i32, _c_i64,    # parents, cu_seqlens, num_seqs, num_tokens
+        _c_p, _c_i32, _c_p,            # tree_mask, mask_words, stream
     ]),
 }
 

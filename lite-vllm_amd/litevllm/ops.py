@@ -819,3 +819,372 @@ def linear_if_plain(x: torch.Tensor, weight: torch.Tensor,
 def linear_f32_if_plain(x: torch.Tensor, weight: torch.Tensor) -> Optional[torch.Tensor]:
     """linear_if_plain for fp32 operands; None for others."""
     return linear_if_plain(x, weight) if x.dtype is torch.float32 else None
+
+
+# ---------------------------------------------------------------------------
+# 8-bit paged K/V cache
+# ---------------------------------------------------------------------------
+
+_CODES = {torch.int8: _hip.LV_INT8, torch.float8_e4m3fn: _hip.LV_E4M3}
+QUANT_DTYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+
+
+class QuantKV(NamedTuple):
+    """An 8-bit paged cache: codes (int8 or float8_e4m3fn) [num_blocks,
+    block_size, num_kv_heads, head_dim] and one fp32 scale for each token and
+    kv head; a cached value is code * scale.  Any strides with head_dim
+    innermost (the others multiples of 16); keys and values share them."""
+    key: torch.Tensor
+    value: torch.Tensor
+    key_scale: torch.Tensor      # float32 [num_blocks, block_size, num_kv_heads]
+    value_scale: torch.Tensor
+
+
+def quant_kv_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
+                   dtype: torch.dtype, device) -> QuantKV:
+    """An empty 8-bit cache (all values 0), each head's rows of a block in one
+    run of memory, as the attention kernels read it fastest."""
+    if dtype not in _CODES:
+        raise RuntimeError(f"unsupported cache dtype {dtype}; expected int8 or float8_e4m3fn")
+    codes = torch.zeros((2, num_blocks, num_kv_heads, block_size, head_dim), dtype=torch.int8,
+                        device=device).view(dtype).transpose(2, 3)
+    scales = torch.zeros((2, num_blocks, num_kv_heads, block_size), dtype=torch.float32,
+                         device=device).transpose(2, 3)
+    return QuantKV(codes[0], codes[1], scales[0], scales[1])
+
+
+def _quant_cache(cache: QuantKV) -> _hip.QuantCache:
+    """The C description of a cache, its tensors checked."""
+    key, value, ks, vs = cache
+    dev = key.device
+    for n, t in zip(QuantKV._fields, cache):
+        _require_device(f"cache.{n}", t, dev)
+    if key.dtype not in _CODES or value.dtype != key.dtype:
+        raise RuntimeError(f"cache codes must be int8 or float8_e4m3fn, got {key.dtype} and "
+                           f"{value.dtype}")
+    if key.dim() != 4 or value.shape != key.shape or ks.shape != key.shape[:3] \
+            or vs.shape != ks.shape:
+        raise RuntimeError("cache codes must be [num_blocks, block_size, num_kv_heads, head_dim] "
+                           "and its scales [num_blocks, block_size, num_kv_heads]")
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise RuntimeError("cache scales must be float32")
+    if key.stride(3) != 1 or value.stride() != key.stride() or vs.stride() != ks.stride():
+        raise RuntimeError("cache key and value must share their strides, head_dim innermost")
+    n, bs, hkv, d = key.shape
+    return _hip.QuantCache(_ptr(key), _ptr(value), _ptr(ks), _ptr(vs), n, *key.stride()[:3],
+                           *ks.stride(), bs, hkv, d, _CODES[key.dtype])
+
+
+def _check_heads(name: str, t: torch.Tensor, shape: tuple) -> None:
+    if tuple(t.shape) != shape:
+        raise RuntimeError(f"`{name}` shape {tuple(t.shape)} != {shape}")
+    if t.numel() and (t.stride(2) != 1 or t.stride(1) != shape[2]):
+        raise RuntimeError(f"`{name}` must have contiguous heads (strides {t.stride()})")
+
+
+def kv_scatter_quant(key: torch.Tensor, value: torch.Tensor, cache: QuantKV,
+                     slot_mapping: torch.Tensor) -> None:
+    """kv_scatter into an 8-bit cache, in place: row t of key / value [T, Hkv,
+    D] (fp32, fp16 or bf16) becomes D codes and a scale at slot_mapping[t].
+
+    Reference: litevllm/layers/attention.py:17-33 and 79-84.
+    """
+    c = _quant_cache(cache)
+    dev = cache.key.device
+    for n, t in (("key", key), ("value", value), ("slot_mapping", slot_mapping)):
+        _require_device(n, t, dev)
+    _check_int("slot_mapping", slot_mapping, torch.int64, 1)
+    T = slot_mapping.shape[0]
+    if value.dtype != key.dtype:
+        raise RuntimeError(f"key and value dtypes differ: {key.dtype}, {value.dtype}")
+    for n, t in (("key", key), ("value", value)):
+        _check_heads(n, t, (T, c.num_kv_heads, c.head_dim))
+    if T == 0:
+        return
+    rc = _hip.load().lv_kv_scatter_quant(_ptr(key), key.stride(0), _ptr(value), value.stride(0), c,
+                                         _ptr(slot_mapping), T, _dtype_code(key), _stream(dev))
+    _hip.check(rc, "lv_kv_scatter_quant")
+
+
+def kv_gather_quant(cache: QuantKV, slots: torch.Tensor, dtype: torch.dtype,
+                    out: Optional[tuple[torch.Tensor, torch.Tensor]] = None
+                    ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(key, value) rows [T, Hkv, D] of an 8-bit cache at the given slots, as
+    values of `dtype`; rows of zeros at negative slots."""
+    c = _quant_cache(cache)
+    dev = cache.key.device
+    _require_device("slots", slots, dev)
+    _check_int("slots", slots, torch.int64, 1)
+    shape = (slots.shape[0], c.num_kv_heads, c.head_dim)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=dtype, device=dev) for _ in range(2))
+    for n, t in zip(("out[0]", "out[1]"), out):
+        _require_device(n, t, dev)
+        _check_heads(n, t, shape)
+        if t.dtype != dtype:
+            raise RuntimeError(f"`{n}` dtype {t.dtype} != {dtype}")
+    code = _dtype_code(out[0])
+    if shape[0] == 0:
+        return out
+    rc = _hip.load().lv_kv_gather_quant(c, _ptr(slots), shape[0], _ptr(out[0]), out[0].stride(0),
+                                        _ptr(out[1]), out[1].stride(0), code, _stream(dev))
+    _hip.check(rc, "lv_kv_gather_quant")
+    return out
+
+
+def qk_norm_rope_cache_quant(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
+                             cos_cache: torch.Tensor, sin_cache: torch.Tensor,
+                             positions: torch.Tensor, slot_mapping: torch.Tensor, cache: QuantKV,
+                             q_norm_weight: Optional[torch.Tensor] = None,
+                             k_norm_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                             q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """qk_norm_rope_cache with K and V written into an 8-bit cache.  Rows stay
+    in fp32 up to the query's one rounding and the codes.
+
+    Reference: models/qwen3.py:75-84, layers/rotary_emb.py:92-117,
+    layers/attention.py:79-84.
+    """
+    c = _quant_cache(cache)
+    dev = cache.key.device
+    for n, t in (("qkv", qkv), ("cos_cache", cos_cache), ("sin_cache", sin_cache),
+                 ("positions", positions), ("slot_mapping", slot_mapping),
+                 ("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight),
+                 ("q_out", q_out)):
+        _require_device(n, t, dev)
+    H, Hkv, D = num_heads, num_kv_heads, head_dim
+    if (c.num_kv_heads, c.head_dim) != (Hkv, D):
+        raise RuntimeError(f"cache has {c.num_kv_heads} kv heads of {c.head_dim} dims, expected "
+                           f"{Hkv} of {D}")
+    _check_rows("qkv", qkv, (H + 2 * Hkv) * D, qkv.dtype)
+    T = qkv.shape[0]
+    _check_int("positions", positions, torch.int64, 1)
+    _check_int("slot_mapping", slot_mapping, torch.int64, 1)
+    if positions.shape[0] != T or slot_mapping.shape[0] != T:
+        raise RuntimeError("positions / slot_mapping length != number of tokens")
+    for n, t in (("cos_cache", cos_cache), ("sin_cache", sin_cache)):
+        if t.dim() != 2 or t.shape[1] != D // 2 or not t.is_contiguous() or t.dtype != qkv.dtype:
+            raise RuntimeError(f"`{n}` must be a contiguous [max_pos, {D // 2}] {qkv.dtype} tensor")
+    if sin_cache.shape != cos_cache.shape:
+        raise RuntimeError("cos_cache and sin_cache shapes differ")
+    for n, t in (("q_norm_weight", q_norm_weight), ("k_norm_weight", k_norm_weight)):
+        if t is not None and (t.shape != (D,) or not t.is_contiguous() or t.dtype != qkv.dtype):
+            raise RuntimeError(f"`{n}` must be a contiguous [{D}] {qkv.dtype} tensor")
+    if q_out is None:
+        q_out = torch.empty((T, H, D), dtype=qkv.dtype, device=dev)
+    _check_heads("q_out", q_out, (T, H, D))
+    if q_out.dtype != qkv.dtype:
+        raise RuntimeError(f"`q_out` dtype {q_out.dtype} != {qkv.dtype}")
+    code = _dtype_code(qkv)
+    if T == 0:
+        return q_out
+    rc = _hip.load().lv_qk_norm_rope_cache_quant(
+        _ptr(qkv), qkv.stride(0), _ptr(q_norm_weight), _ptr(k_norm_weight), _ptr(cos_cache),
+        _ptr(sin_cache), cos_cache.shape[0], _ptr(positions), _ptr(slot_mapping), _ptr(q_out),
+        q_out.stride(0), c, T, H, float(eps), code, _stream(dev))
+    _hip.check(rc, "lv_qk_norm_rope_cache_quant")
+    return q_out
+
+
+def _attention_args(query, dev, block_tables, context_lens, cu_seqlens, out):
+    """The checks common to the attention calls below; returns out."""
+    for n, t in (("query", query), ("block_tables", block_tables), ("context_lens", context_lens),
+                 ("cu_seqlens", cu_seqlens), ("out", out)):
+        _require_device(n, t, dev)
+    if query.dim() != 3:
+        raise RuntimeError(f"query must be [T, H, D], got {tuple(query.shape)}")
+    _check_heads("query", query, tuple(query.shape))
+    _check_int("block_tables", block_tables, torch.int32, 2)
+    _check_int("context_lens", context_lens, torch.int32, 1)
+    B = block_tables.shape[0]
+    if context_lens.shape[0] != B:
+        raise RuntimeError("context_lens and block_tables disagree on the batch size")
+    if cu_seqlens is not None:
+        _check_int("cu_seqlens", cu_seqlens, torch.int32, 1)
+        if cu_seqlens.shape[0] != B + 1:
+            raise RuntimeError("cu_seqlens must have num_seqs + 1 entries")
+    elif query.shape[0] != B:
+        raise RuntimeError("without cu_seqlens every sequence must have exactly one query row")
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    elif out.dtype != query.dtype:
+        raise RuntimeError("`out` must have query's dtype")
+    _check_heads("out", out, tuple(query.shape))
+    return out
+
+
+def _given_workspace(workspace, need: int, dev):
+    """The caller's workspace, or the stream's scratch buffer."""
+    if workspace is None:
+        return _workspace(dev, need)
+    _require_device("workspace", workspace, dev)
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+        raise RuntimeError(f"workspace must be a contiguous uint8 tensor of >= {need} bytes")
+    return workspace if workspace.numel() > 0 else None
+
+
+def paged_attention_quant(query: torch.Tensor, cache: QuantKV, block_tables: torch.Tensor,
+                          context_lens: torch.Tensor, *, scale: float,
+                          cu_seqlens: Optional[torch.Tensor] = None,
+                          num_decodes: Optional[int] = None, max_query_len: int = 1,
+                          out: Optional[torch.Tensor] = None,
+                          workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_attention over an 8-bit cache: query [T, H, D] (fp32, fp16 or
+    bf16), decode rows first, then causal chunks.
+
+    Reference: litevllm/layers/attention.py:91-151.
+    """
+    c = _quant_cache(cache)
+    dev = cache.key.device
+    out = _attention_args(query, dev, block_tables, context_lens, cu_seqlens, out)
+    T, H, D = query.shape
+    if D != c.head_dim:
+        raise RuntimeError(f"cache head_dim {c.head_dim} does not match the query's {D}")
+    B, max_blocks = block_tables.shape
+    if num_decodes is None:
+        num_decodes = B if cu_seqlens is None else 0
+    dt = _dtype_code(query)
+    if B == 0 or T == 0:
+        return out
+    lib = _hip.load()
+    need = lib.lv_paged_attention_quant_workspace_size(B, num_decodes, T, max_query_len, H,
+                                                       c.num_kv_heads, D, max_blocks, dt)
+    ws = _given_workspace(workspace, need, dev)
+    rc = lib.lv_paged_attention_quant(
+        _ptr(query), query.stride(0), c, _ptr(block_tables), max_blocks, _ptr(cu_seqlens),
+        _ptr(context_lens), B, num_decodes, T, max_query_len, H, float(scale), _ptr(out),
+        out.stride(0), _ptr(ws), 0 if ws is None else ws.numel(), dt, _stream(dev))
+    _hip.check(rc, "lv_paged_attention_quant")
+    return out
+
+
+def paged_attention_quant_workspace_size(num_seqs: int, num_decodes: int, num_tokens: int,
+                                         max_query_len: int, num_heads: int, num_kv_heads: int,
+                                         head_dim: int, max_blocks: int,
+                                         dtype: torch.dtype) -> int:
+    """Bytes of scratch one paged_attention_quant call with these sizes needs."""
+    return int(_hip.load().lv_paged_attention_quant_workspace_size(
+        num_seqs, num_decodes, num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
+        max_blocks, _DTYPE_CODES[dtype]))
+
+
+# ---------------------------------------------------------------------------
+# trees of drafted tokens
+# ---------------------------------------------------------------------------
+
+def tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor, max_query_len: int) -> torch.Tensor:
+    """Ancestor bits int64 [T, ceil(max_query_len / 64)] of drafted trees, for
+    tree_attention: bit t % 64 of word t // 64 of a row says that its token
+    sees drafted token t of its sequence (itself and its ancestors).
+    ``parents``: int32 [T], each token's parent among its sequence's drafted
+    tokens (smaller than its own index), or -1."""
+    dev = parents.device
+    _require_device("parents", parents, dev)
+    _require_device("cu_seqlens", cu_seqlens, dev)
+    _check_int("parents", parents, torch.int32, 1)
+    _check_int("cu_seqlens", cu_seqlens, torch.int32, 1)
+    words = max(1, -(-int(max_query_len) // 64))
+    T, B = parents.shape[0], cu_seqlens.shape[0] - 1
+    mask = torch.zeros((T, words), dtype=torch.int64, device=dev)
+    if T == 0 or B <= 0:
+        return mask
+    rc = _hip.load().lv_tree_mask(_ptr(parents), _ptr(cu_seqlens), B, T, _ptr(mask), words,
+                                  _stream(dev))
+    _hip.check(rc, "lv_tree_mask")
+    return mask
+
+
+def _check_tree(query, tree_mask, cu_seqlens, max_query_len, dev) -> int:
+    _require_device("tree_mask", tree_mask, dev)
+    if cu_seqlens is None:
+        raise RuntimeError("tree attention needs cu_seqlens")
+    _check_int("tree_mask", tree_mask, torch.int64, 2)
+    T, words = tree_mask.shape
+    if T != query.shape[0] or words * 64 < max_query_len or words < 1:
+        raise RuntimeError(f"tree_mask must be [{query.shape[0]}, >= {-(-max_query_len // 64)}], "
+                           f"got {tuple(tree_mask.shape)}")
+    return words
+
+
+def tree_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                   block_tables: torch.Tensor, context_lens: torch.Tensor,
+                   cu_seqlens: torch.Tensor, tree_mask: torch.Tensor, *, scale: float,
+                   max_query_len: int, out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted token trees over the paged cache: the rows
+    cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of query [T, H, D] are sequence i's
+    drafted tokens, whose K/V are in the cache behind its committed tokens
+    (context_lens counts both).  Each row sees every committed key and the
+    drafted ones of its tree_mask row (see tree_mask); a row that sees nothing
+    is zeros.
+
+    The reference decodes one token per sequence and step
+    (litevllm/layers/attention.py:91-139).
+    """
+    dev = key_cache.device
+    for n, t in (("key_cache", key_cache), ("value_cache", value_cache)):
+        _require_device(n, t, dev)
+    out = _attention_args(query, dev, block_tables, context_lens, cu_seqlens, out)
+    words = _check_tree(query, tree_mask, cu_seqlens, max_query_len, dev)
+    T, H, D = query.shape
+    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape \
+            or not key_cache.is_contiguous() or not value_cache.is_contiguous():
+        raise RuntimeError("caches must be contiguous [num_blocks, block_size, num_kv_heads, head_dim]")
+    n_blocks, bs, hkv, d = key_cache.shape
+    if d != D or query.dtype != key_cache.dtype or value_cache.dtype != key_cache.dtype:
+        raise RuntimeError("query and caches must share one head_dim and dtype")
+    dt = _dtype_code(query)
+    B, max_blocks = block_tables.shape
+    if B == 0 or T == 0:
+        return out
+    lib = _hip.load()
+    need = lib.lv_tree_attention_workspace_size(B, T, max_query_len, H, hkv, D, max_blocks, dt)
+    ws = _given_workspace(workspace, need, dev)
+    rc = lib.lv_tree_attention(
+        _ptr(query), query.stride(0), _ptr(key_cache), _ptr(value_cache), n_blocks,
+        _ptr(block_tables), max_blocks, _ptr(cu_seqlens), _ptr(context_lens), _ptr(tree_mask),
+        words, B, T, max_query_len, H, hkv, D, bs, float(scale), _ptr(out), out.stride(0), _ptr(ws),
+        0 if ws is None else ws.numel(), dt, _stream(dev))
+    _hip.check(rc, "lv_tree_attention")
+    return out
+
+
+def tree_attention_quant(query: torch.Tensor, cache: QuantKV, block_tables: torch.Tensor,
+                         context_lens: torch.Tensor, cu_seqlens: torch.Tensor,
+                         tree_mask: torch.Tensor, *, scale: float, max_query_len: int,
+                         out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """tree_attention over an 8-bit cache.
+
+    Reference: litevllm/layers/attention.py:91-139.
+    """
+    c = _quant_cache(cache)
+    dev = cache.key.device
+    out = _attention_args(query, dev, block_tables, context_lens, cu_seqlens, out)
+    words = _check_tree(query, tree_mask, cu_seqlens, max_query_len, dev)
+    T, H, D = query.shape
+    if D != c.head_dim:
+        raise RuntimeError(f"cache head_dim {c.head_dim} does not match the query's {D}")
+    dt = _dtype_code(query)
+    B, max_blocks = block_tables.shape
+    if B == 0 or T == 0:
+        return out
+    lib = _hip.load()
+    need = lib.lv_tree_attention_workspace_size(B, T, max_query_len, H, c.num_kv_heads, D,
+                                                max_blocks, dt)
+    ws = _given_workspace(workspace, need, dev)
+    rc = lib.lv_tree_attention_quant(
+        _ptr(query), query.stride(0), c, _ptr(block_tables), max_blocks, _ptr(cu_seqlens),
+        _ptr(context_lens), _ptr(tree_mask), words, B, T, max_query_len, H, float(scale),
+        _ptr(out), out.stride(0), _ptr(ws), 0 if ws is None else ws.numel(), dt, _stream(dev))
+    _hip.check(rc, "lv_tree_attention_quant")
+    return out
+
+
+def tree_attention_workspace_size(num_seqs: int, num_tokens: int, max_query_len: int,
+                                  num_heads: int, num_kv_heads: int, head_dim: int,
+                                  max_blocks: int, dtype: torch.dtype) -> int:
+    """Bytes of scratch one tree_attention (or tree_attention_quant) call with
+    these sizes needs."""
+    return int(_hip.load().lv_tree_attention_workspace_size(
+        num_seqs, num_tokens, max_query_len, num_heads, num_kv_heads, head_dim, max_blocks,
+        _DTYPE_CODES[dtype]))
