@@ -8,75 +8,12 @@
 //   x_t = scale * s_t * (q . c_t),   o = sum_t w_t s'_t c'_t / sum_t w_t,
 //   w_t = exp(x_t - max)
 // with the codes taken as they are and the scales applied to fp32 values.
-#include <type_traits>
+#include <algorithm>
+#include <atomic>
 
-#include "lv_common.h"
-#include "lv_quant.h"
+#include "kv_attention.h"
 
 namespace lv {
-
-// A paged cache of element or code type; strides in elements.
-struct KvView {
-  const void* kv[2];
-  const float* scale[2];         // 8-bit caches only
-  int64_t blk, tok, head;
-  int64_t sblk, stok, shead;
-  int64_t num_blocks;
-};
-
-struct Batch {
-  const int32_t* block_tables; int max_blocks;
-  const int32_t* cu; const int32_t* ctx;
-  const uint64_t* mask; int mask_words;      // trees only
-  int num_seqs; int num_tokens;
-};
-
-struct Rows {
-  const void* q; int64_t q_stride;
-  void* out; int64_t out_stride;
-  int num_heads, num_kv_heads;
-  float scale_log2;
-};
-
-constexpr int kBs = 16;
-constexpr float kNegBig = -1.0e30f;
-
-template <typename C> struct cached {          // 8-bit codes
-  static constexpr bool kCodes = true;
-  static constexpr int kBytes = 1;
-  static constexpr int kPer16B = 16;
-  __device__ __forceinline__ static void unpack(const uint4& v, float* out) {
-    code<C>::unpack4(v.x, out);
-    code<C>::unpack4(v.y, out + 4);
-    code<C>::unpack4(v.z, out + 8);
-    code<C>::unpack4(v.w, out + 12);
-  }
-};
-template <typename T> struct cached_elem : elem<T> { static constexpr bool kCodes = false; };
-template <> struct cached<float> : cached_elem<float> {};
-template <> struct cached<f16> : cached_elem<f16> {};
-template <> struct cached<bf16> : cached_elem<bf16> {};
-
-// A sequence's query rows [q0, q0 + n) and its keys [0, ctx), clamped to the
-// batch's tensors.
-struct Seq { int q0, n, ctx; };
-__device__ __forceinline__ Seq sequence(const Batch& b, int i) {
-  Seq s;
-  s.q0 = b.cu ? b.cu[i] : i;
-  const int q1 = b.cu ? b.cu[i + 1] : i + 1;
-  s.q0 = min(max(s.q0, 0), b.num_tokens);
-  s.n = min(max(q1 - s.q0, 0), b.num_tokens - s.q0);
-  s.ctx = min(max(b.ctx[i], 0), b.max_blocks * kBs);
-  return s;
-}
-
-__device__ __forceinline__ int physical_block(const Batch& b, int64_t num_blocks, int seq,
-                                              int blk) {
-  const int id = b.block_tables[(int64_t)seq * b.max_blocks + blk];
-  if (id >= 0 && id < num_blocks) return id;
-  report_device_error(LV_DEVERR_BLOCK_ID);     // clamped and reported
-  return 0;
-}
 
 // One workgroup of 4 wavefronts per (query row, head).  A lane takes one key
 // of 64 for the scores (its whole row, against the query in LDS), then one or
@@ -222,13 +159,6 @@ LV_ERROR_WORD_READER(read_errors_tree)
 // ---------------------------------------------------------------------------
 namespace {
 
-struct Call {
-  Batch b; KvView c; Rows r;
-  int d; lv_dtype dtype; int code;     // code: lv_code, or -1 for a cache of dtype
-  bool tree;
-  hipStream_t stream;
-};
-
 template <typename T, typename C, int D>
 int launch_rows(const Call& a) {
   const dim3 grid((unsigned)a.b.num_tokens, (unsigned)a.r.num_heads);
@@ -237,31 +167,90 @@ int launch_rows(const Call& a) {
   return check_launch("attn_row_kernel");
 }
 
-template <typename T, typename C>
-int launch_d(const Call& a) {
-  return a.d == 64 ? launch_rows<T, C, 64>(a) : launch_rows<T, C, 128>(a);
+int launch_rows(const Call& a) {      // an fp32 cache
+  return a.d == 64 ? launch_rows<float, float, 64>(a) : launch_rows<float, float, 128>(a);
 }
 
-template <typename T>
-int launch_c(const Call& a) {
-  if (a.code == LV_INT8) return launch_d<T, int8_code>(a);
-  if (a.code == LV_E4M3) return launch_d<T, e4m3_code>(a);
-  return launch_d<T, T>(a);
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// CUs of the current device (looked up once per device).
+int device_cus() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  n = known[dev].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
+    n = 256;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
-int launch(const Call& a) {
-  if (a.dtype == LV_F32) return launch_c<float>(a);
-  if (a.dtype == LV_F16) return launch_c<f16>(a);
-  return launch_c<bf16>(a);
+// How the sequences of a part are launched.  Everything here follows from the
+// sizes the caller names, never from what is in device memory.
+TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num_kv_heads,
+                    int head_dim, int max_blocks, lv_dtype dtype) {
+  TilePlan p{};
+  p.seq_begin = seq_begin;
+  p.n_seqs = n_seqs;
+  p.max_q = max_q;
+  const int64_t rows = std::max<int64_t>(1, (int64_t)max_q * (num_heads / num_kv_heads));
+  p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  const int r = 32 * p.rw, kt = p.rw == 4 ? 64 : 128;
+  const int64_t units = (int64_t)n_seqs * num_kv_heads * ((rows + r - 1) / r);
+  const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_blocks * kBs + kt - 1) / kt);
+  // contexts of a few tiles: splitting them costs more than it gives
+  p.whole = tiles <= 4;
+  const int64_t resident = (int64_t)device_cus() * (dtype == LV_F32 ? 1 : 2);
+  p.grid = (int)(p.whole ? std::min<int64_t>(units, 1 << 20)
+                         : std::min<int64_t>(units * tiles, resident));
+  p.slot_rows = (int)std::min<int64_t>(rows, r);
+  if (!p.whole) {
+    p.head_bytes = align256((size_t)p.grid * 2 * 16);
+    p.ml_bytes = align256((size_t)2 * p.grid * p.slot_rows * 8);
+    p.acc_bytes = align256((size_t)2 * p.grid * p.slot_rows * head_dim * 4);
+  }
+  return p;
 }
 
-size_t workspace_size(int64_t num_tokens, int max_query_len, int num_heads, int num_kv_heads,
-                      int head_dim, int max_blocks) {
-  return 0;
+size_t plan_bytes(const TilePlan& p) { return p.head_bytes + p.ml_bytes + p.acc_bytes; }
+
+size_t workspace_size(int num_seqs, int num_decodes, int max_query_len, int num_heads,
+                      int num_kv_heads, int head_dim, int max_blocks, lv_dtype dtype) {
+  if (num_seqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || max_blocks < 0) return 0;
+  size_t need = 0;
+  if (num_decodes > 0)
+    need = plan_bytes(plan_tiles(0, num_decodes, 1, num_heads, num_kv_heads, head_dim, max_blocks,
+                                 dtype));
+  if (num_seqs > num_decodes)
+    need = std::max(need, plan_bytes(plan_tiles(num_decodes, num_seqs - num_decodes,
+                                                max_query_len, num_heads, num_kv_heads, head_dim,
+                                                max_blocks, dtype)));
+  return need;
+}
+
+int launch_part(const Call& a, const TilePlan& p, char* ws) {
+  if (a.dtype == LV_F32) return launch_tiles_f32(a, p, ws);
+  if (a.dtype == LV_F16) return launch_tiles_f16(a, p, ws);
+  return launch_tiles_bf16(a, p, ws);
+}
+
+int launch(const Call& a, int num_decodes, int max_query_len, void* ws) {
+  const int h = a.r.num_heads, hkv = a.r.num_kv_heads, mb = a.b.max_blocks;
+  if (a.code < 0 && a.dtype == LV_F32) return launch_rows(a);
+  if (num_decodes > 0)
+    if (const int rc = launch_part(a, plan_tiles(0, num_decodes, 1, h, hkv, a.d, mb, a.dtype),
+                                   (char*)ws);
+        rc != LV_OK)
+      return rc;
+  if (num_decodes == a.b.num_seqs) return LV_OK;
+  return launch_part(a, plan_tiles(num_decodes, a.b.num_seqs - num_decodes, max_query_len, h, hkv,
+                                   a.d, mb, a.dtype),
+                     (char*)ws);
 }
 
 // The checks common to the attention entries; fills `a` but for the cache.
-int check_call(const char* who, Call& a, const void* query, int64_t q_stride,
+int check_call(const char* who, Call& a, int num_decodes, const void* query, int64_t q_stride,
                const int32_t* tables, int max_blocks, const int32_t* cu, const int32_t* ctx,
                int num_seqs, int64_t num_tokens, int max_query_len, int num_heads,
                int num_kv_heads, int head_dim, int block_size, float scale, void* out,
@@ -296,8 +285,17 @@ int check_call(const char* who, Call& a, const void* query, int64_t q_stride,
   a.r.num_heads = num_heads; a.r.num_kv_heads = num_kv_heads;
   a.r.scale_log2 = scale * 1.4426950408889634f;
   a.d = head_dim; a.dtype = dtype;
-  const size_t need = workspace_size(num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
-                                     max_blocks);
+  const int64_t g = num_heads / num_kv_heads;
+  const int64_t units = (int64_t)num_seqs * num_kv_heads * ((max_query_len * g + 31) / 32);
+  LV_REQUIRE(units * std::max(1, max_blocks / 4 + 1) < (1ll << 31) - (1 << 16) &&
+                 max_query_len * g < (1ll << 30),
+             "%s: too many keys and rows for 32-bit offsets", who);
+  if (num_seqs > 16384) {
+    set_error("%s: %d sequences (up to 16384 are supported)", who, num_seqs);
+    return LV_ERR_UNSUPPORTED;
+  }
+  const size_t need = workspace_size(num_seqs, num_decodes, max_query_len, num_heads, num_kv_heads,
+                                     head_dim, max_blocks, dtype);
   if (need > 0 && (!ws || ((uintptr_t)ws & 255) != 0 || ws_bytes < need)) {
     set_error("%s: workspace of %zu bytes (256-byte aligned) needed, got %zu", who, need,
               ws ? ws_bytes : (size_t)0);
@@ -334,16 +332,16 @@ extern "C" size_t lv_paged_attention_quant_workspace_size(int32_t num_seqs, int3
                                                           int32_t num_heads,
                                                           int32_t num_kv_heads, int32_t head_dim,
                                                           int32_t max_blocks, lv_dtype dtype) {
-  return lv::workspace_size(num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
-                            max_blocks);
+  return lv::workspace_size(num_seqs, num_decodes, max_query_len, num_heads, num_kv_heads,
+                            head_dim, max_blocks, dtype);
 }
 
 extern "C" size_t lv_tree_attention_workspace_size(int32_t num_seqs, int64_t num_tokens,
                                                    int32_t max_query_len, int32_t num_heads,
                                                    int32_t num_kv_heads, int32_t head_dim,
                                                    int32_t max_blocks, lv_dtype dtype) {
-  return lv::workspace_size(num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
-                            max_blocks);
+  return lv::workspace_size(num_seqs, 0, max_query_len, num_heads, num_kv_heads, head_dim,
+                            max_blocks, dtype);
 }
 
 extern "C" int lv_paged_attention_quant(
@@ -359,7 +357,7 @@ extern "C" int lv_paged_attention_quant(
   LV_REQUIRE(num_decodes >= 0 && num_decodes <= num_seqs && num_decodes <= num_tokens,
              "%s: num_decodes %d outside [0, num_seqs]", who, num_decodes);
   Call a{};
-  if (const int rc = check_call(who, a, query_dev, q_stride_t, block_tables_dev, max_blocks,
+  if (const int rc = check_call(who, a, num_decodes, query_dev, q_stride_t, block_tables_dev, max_blocks,
                                 cu_seqlens_dev, context_lens_dev, num_seqs, num_tokens,
                                 max_query_len, num_heads, cache->num_kv_heads, cache->head_dim,
                                 cache->block_size, scale, out_dev, out_stride_t, workspace_dev,
@@ -368,7 +366,7 @@ extern "C" int lv_paged_attention_quant(
     return rc;
   use_cache(a, cache);
   a.stream = (hipStream_t)stream;
-  return launch(a);
+  return launch(a, num_decodes, max_query_len, workspace_dev);
 }
 
 extern "C" int lv_tree_attention(
@@ -387,7 +385,7 @@ extern "C" int lv_tree_attention(
       rc != LV_OK)
     return rc;
   LV_REQUIRE(num_cache_blocks > 0, "%s: bad cache geometry", who);
-  if (const int rc = check_call(who, a, query_dev, q_stride_t, block_tables_dev, max_blocks,
+  if (const int rc = check_call(who, a, 0, query_dev, q_stride_t, block_tables_dev, max_blocks,
                                 cu_seqlens_dev, context_lens_dev, num_seqs, num_tokens,
                                 max_query_len, num_heads, num_kv_heads, head_dim, block_size,
                                 scale, out_dev, out_stride_t, workspace_dev, workspace_bytes,
@@ -403,7 +401,7 @@ extern "C" int lv_tree_attention(
                0, 0, 0, num_cache_blocks};
   a.code = -1;
   a.stream = (hipStream_t)stream;
-  return launch(a);
+  return launch(a, 0, max_query_len, workspace_dev);
 }
 
 extern "C" int lv_tree_attention_quant(
@@ -421,7 +419,7 @@ extern "C" int lv_tree_attention_quant(
   if (const int rc = check_mask(who, a, tree_mask_dev, mask_words, max_query_len, num_tokens);
       rc != LV_OK)
     return rc;
-  if (const int rc = check_call(who, a, query_dev, q_stride_t, block_tables_dev, max_blocks,
+  if (const int rc = check_call(who, a, 0, query_dev, q_stride_t, block_tables_dev, max_blocks,
                                 cu_seqlens_dev, context_lens_dev, num_seqs, num_tokens,
                                 max_query_len, num_heads, cache->num_kv_heads, cache->head_dim,
                                 cache->block_size, scale, out_dev, out_stride_t, workspace_dev,
@@ -431,7 +429,7 @@ extern "C" int lv_tree_attention_quant(
   LV_REQUIRE(cu_seqlens_dev, "%s: null cu_seqlens", who);
   use_cache(a, cache);
   a.stream = (hipStream_t)stream;
-  return launch(a);
+  return launch(a, 0, max_query_len, workspace_dev);
 }
 
 extern "C" int lv_tree_mask(const int32_t* parents_dev, const int32_t* cu_seqlens_dev,

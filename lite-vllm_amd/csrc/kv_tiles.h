@@ -1,0 +1,853 @@
+// Attention over paged caches on the matrix cores (the kernel and its launch;
+// included by one translation unit per query type).
+#pragma once
+#include "kv_attention.h"
+#include "lv_attn.h"
+#include "lv_mfma.h"
+
+namespace lv {
+
+// ---------------------------------------------------------------------------
+// Tiles on the matrix cores.
+//
+// The query rows of a sequence that read one kv head are its (token, head of
+// the group) pairs; a unit is up to R = 32 RW of them and the keys they need,
+// in tiles of KT.  All units' tiles form one list, which a fixed grid of
+// workgroups splits into equal contiguous ranges: the work is even however
+// unlike the contexts are, and nothing about them has to be known on the
+// host.  A unit inside one range is written to `out`; the pieces of one that
+// spans several go to the workspace (m, l, O / l in fp32) and attn_join_kernel
+// joins them.
+//
+// A workgroup is 4 wavefronts: RW groups of 32 rows times KW = 4 / RW parts
+// of every tile's keys, so that few rows (RW = 1: decodes, small trees) still
+// use four wavefronts; the KW states are merged through LDS when a piece ends.
+// Per tile:
+//   * the next tile's rows are loaded from HBM into registers while this one
+//     is computed, then turned into 16-bit operands (codes are exact in bf16
+//     and fp16) and written to LDS, swizzled (ChunkLds);
+//   * S^T = K Q^T, v_mfma_f32_32x32x16: a lane ends with one query row (its
+//     column) against 16 of each 32 keys;
+//   * x = S^T * (scale of the key's row * scale), masked by position or tree;
+//     running maximum (raised only when passed by 2^8), weights and their sum
+//     in fp32;
+//   * O^T += V^T P^T with P = weight * scale of the value's row.  P is split
+//     into PP bf16 (fp16 cache: fp16) parts, each a product of its own: two
+//     hold 16 bits (2^-17 of a weight), three all of fp32.  One part (2^-9)
+//     would add an error as large as the output's own rounding.
+// fp32 queries are three bf16 parts (all their bits), others are taken as
+// they are.
+//
+// Zero weights times a value that is not finite make NaN: a piece whose sums
+// are not finite is computed again key by key (careful), where a key that a
+// row does not see is not read.
+// ---------------------------------------------------------------------------
+constexpr int kTileThreads = 256;
+
+struct TileArgs {
+  Batch b; KvView c; Rows r;
+  int seq_begin, n_seqs, max_q;
+  int whole;                // ranges of whole units: nothing to join
+  int slot_rows;            // rows of a workspace slot
+  int4* head;               // [grid][2]: the unit that crosses a range's start
+  float* ml;                // [2 grid][slot_rows][2]
+  float* acc;               // [2 grid][slot_rows][D]
+};
+
+struct Unit { int seq, q0, n, rows, committed, kend, kvh, row0, ntiles; };
+
+template <int RW> struct TileCfg {
+  static constexpr int R = 32 * RW, KW = 4 / RW;
+  static constexpr int KT = RW == 4 ? 64 : 128;   // keys per tile
+  static constexpr int BPW = KT / 64;             // 16-token blocks a wavefront stages
+  static constexpr int KPW = KT / KW;             // keys a wavefront computes
+};
+
+// Keys that row tile [row0, row0 + R) of a sequence needs.
+template <bool TREE, int R>
+__device__ __forceinline__ int keys_needed(int ctx, int committed, int rows, int row0, int g) {
+  if (TREE) return ctx;
+  return max(0, min(ctx, committed + (min(row0 + R, rows) - 1) / g + 1));
+}
+
+__device__ __forceinline__ Seq tile_sequence(const TileArgs& a, int i) {
+  return sequence(a.b, a.seq_begin + i);
+}
+
+// Tiles of sequence i, over all its row tiles and kv heads.
+template <bool TREE, int RW>
+__device__ __forceinline__ int sequence_tiles(const TileArgs& a, int i, int g) {
+  using F = TileCfg<RW>;
+  const Seq s = tile_sequence(a, i);
+  const int rows = min(s.n, a.max_q) * g;
+  int sum = 0;
+  if (TREE || a.whole) {
+    sum = (rows + F::R - 1) / F::R * (a.whole ? 1 : max(1, (s.ctx + F::KT - 1) / F::KT));
+  } else {
+    for (int r0 = 0; r0 < rows; r0 += F::R)
+      sum += max(1, (keys_needed<TREE, F::R>(s.ctx, s.ctx - s.n, rows, r0, g) + F::KT - 1) / F::KT);
+  }
+  return sum * a.r.num_kv_heads;
+}
+
+// Exclusive scan of the sequences' tiles into off[0 .. n_seqs].
+template <bool TREE, int RW>
+__device__ void scan_tiles(const TileArgs& a, int g, int* off, int* part) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int per = (a.n_seqs + kTileThreads - 1) / kTileThreads;
+  const int lo = min(a.n_seqs, t * per), hi = min(a.n_seqs, lo + per);
+  int sum = 0;
+  for (int i = lo; i < hi; ++i) {
+    off[i] = sum;                       // within the thread's run
+    sum += sequence_tiles<TREE, RW>(a, i, g);
+  }
+  int incl = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(incl, d);
+    if (lane >= d) incl += u;
+  }
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  int base = incl - sum;
+  for (int w = 0; w < wave; ++w) base += part[w];
+  for (int i = lo; i < hi; ++i) off[i] += base;
+  if (t == kTileThreads - 1) off[a.n_seqs] = base + sum;
+  __syncthreads();
+}
+
+template <bool TREE, int RW>
+__device__ __forceinline__ void set_rows(const TileArgs& a, Unit& u, int ctx, int g) {
+  using F = TileCfg<RW>;
+  u.kend = keys_needed<TREE, F::R>(ctx, u.committed, u.rows, u.row0, g);
+  u.ntiles = max(1, (u.kend + F::KT - 1) / F::KT);
+}
+__device__ __forceinline__ int set_seq(const TileArgs& a, Unit& u, int i, int g) {
+  const Seq s = tile_sequence(a, i);
+  u.seq = i; u.q0 = s.q0; u.n = s.n;
+  u.rows = min(s.n, a.max_q) * g;
+  u.committed = s.ctx - s.n;
+  return s.ctx;
+}
+
+// The unit that holds place p of the list, and p's tile in it.
+template <bool TREE, int RW>
+__device__ __forceinline__ int locate(const TileArgs& a, const int* off, int p, int g, Unit& u) {
+  using F = TileCfg<RW>;
+  int lo = 0, hi = a.n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (off[mid] <= p) lo = mid; else hi = mid - 1;
+  }
+  const int ctx = set_seq(a, u, lo, g);
+  const int per_head = (off[lo + 1] - off[lo]) / a.r.num_kv_heads;
+  int rem = p - off[lo];
+  u.kvh = rem / per_head;
+  rem -= u.kvh * per_head;
+  for (u.row0 = 0;; u.row0 += F::R) {
+    set_rows<TREE, RW>(a, u, ctx, g);
+    const int c = a.whole ? 1 : u.ntiles;
+    if (rem < c || u.row0 + F::R >= u.rows) break;
+    rem -= c;
+  }
+  return a.whole ? 0 : rem;
+}
+
+template <bool TREE, int RW>
+__device__ __forceinline__ Unit next_unit(const TileArgs& a, Unit u, int g) {
+  using F = TileCfg<RW>;
+  u.row0 += F::R;
+  int ctx = u.committed + u.n;
+  if (u.row0 >= u.rows) {
+    u.row0 = 0;
+    if (++u.kvh == a.r.num_kv_heads) {
+      u.kvh = 0;
+      do ctx = set_seq(a, u, u.seq + 1, g); while (u.rows == 0 && u.seq + 1 < a.n_seqs);
+    }
+  }
+  set_rows<TREE, RW>(a, u, ctx, g);
+  return u;
+}
+
+// 16 codes -> 16 operands of 16 bits (two 16-byte chunks).
+template <typename O, typename C>
+__device__ __forceinline__ void codes_to_operands(const uint4& w, uint4* out) {
+  const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<C, e4m3_code>::value && std::is_same<O, bf16>::value) {
+      o[2 * i] = __builtin_bit_cast(uint32_t,
+                                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], 1.0f, false));
+      o[2 * i + 1] = __builtin_bit_cast(
+          uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], 1.0f, true));
+    } else if constexpr (std::is_same<C, e4m3_code>::value) {
+      o[2 * i] = __builtin_bit_cast(uint32_t,
+                                    __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(in[i], 1.0f, false));
+      o[2 * i + 1] = __builtin_bit_cast(
+          uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(in[i], 1.0f, true));
+    } else if constexpr (std::is_same<O, bf16>::value) {
+      float f[4];
+      code<C>::unpack4(in[i], f);
+      o[2 * i] = float_to_bf16_pair(f[0], f[1]);
+      o[2 * i + 1] = float_to_bf16_pair(f[2], f[3]);
+    } else {
+      // bytes c + 128 under the exponent of 1024: the fp16 value 1152 + c
+      const uint32_t u = in[i] ^ 0x80808080u;
+      const f16x2_t off = {(_Float16)1152.0f, (_Float16)1152.0f};
+      o[2 * i] = __builtin_bit_cast(
+          uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
+      o[2 * i + 1] = __builtin_bit_cast(
+          uint32_t, __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
+    }
+  }
+  out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// Pairs of fp32 values as their leading bf16 / fp16 parts, taken off them.
+template <typename O>
+__device__ __forceinline__ uint32_t take_part(float& a, float& b, bool last) {
+  if constexpr (std::is_same<O, bf16>::value) {
+    if (last) return float_to_bf16_pair(a, b);
+    const uint32_t w = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+    return w;
+  } else {
+    const uint32_t w = Mfma32<f16>::pack2(a, b);
+    if (!last) {
+      a -= f16_bits_to_float(w & 0xffffu);
+      b -= f16_bits_to_float(w >> 16);
+    }
+    return w;
+  }
+}
+
+__device__ __forceinline__ void team_barrier() {
+  wait_lds();                      // (loads into registers stay in flight)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <typename T, typename C> struct Operands {
+  static constexpr bool kCodes = cached<C>::kCodes;
+  using K = typename std::conditional<std::is_same<T, f16>::value, f16, bf16>::type;
+  using V = typename std::conditional<kCodes, bf16, K>::type;
+  static constexpr int QP = std::is_same<T, float>::value ? 3 : 1;
+  static constexpr int PP = std::is_same<T, float>::value ? 3 : 2;
+  // fp16 weights: the reference lies 2^7 under the maximum that set it, so that
+  // a row's largest weight is between 2^7 and 2^15 and the fixed step of the
+  // smallest fp16 values weighs little against it
+  static constexpr float kLift = std::is_same<V, f16>::value ? 7.0f : 0.0f;
+};
+
+// Workgroups per CU: the three parts of fp32 queries need the registers of two.
+template <typename T> constexpr int kTileWgs = std::is_same<T, float>::value ? 1 : 2;
+
+template <typename T, typename C, int D, int RW, bool TREE>
+__global__ __launch_bounds__(kTileThreads, kTileWgs<T>)
+void attn_tile_kernel(TileArgs a) {
+  using F = TileCfg<RW>;
+  using P = Operands<T, C>;
+  using E = cached<C>;
+  using L = ChunkLds<D, 4>;
+  using KM = Mfma32<typename P::K>;
+  using VM = Mfma32<typename P::V>;
+  constexpr bool kCodes = P::kCodes;
+  constexpr int KT = F::KT, KW = F::KW, KPW = F::KPW, KB = KPW / 32, BPW = F::BPW;
+  constexpr int QSTEPS = D / 16, DBLK = D / 32;
+  constexpr int CPR = D / E::kPer16B;             // 16-byte chunks of a cached row
+  constexpr int RPL = 64 / CPR;                   // rows of a wavefront-wide load
+  constexpr int LPB = kBs / RPL;                  // loads of a block's K or V
+  constexpr int OPC = E::kPer16B / 8;             // operand chunks of a cached chunk
+  static_assert(16 % RPL == 0, "whole loads per block");
+  // K and V tile, then the scales of its keys; the merge of a piece's parts
+  // reuses the tiles (4 wavefronts x 32 rows x D floats at most)
+  extern __shared__ __align__(16) unsigned char s_dyn[];
+  uint16_t* const Ks = reinterpret_cast<uint16_t*>(s_dyn);
+  uint16_t* const Vs = Ks + KT * D;
+  float* const s_ks = reinterpret_cast<float*>(Vs + KT * D);
+  float* const s_vs = s_ks + KT;
+  float2* const s_ml = reinterpret_cast<float2*>(s_vs + KT);   // [4][32]
+  int* const s_off = reinterpret_cast<int*>(s_ml + 128);
+  __shared__ int s_part[4];
+
+  const int H = a.r.num_heads, Hkv = a.r.num_kv_heads;
+  const int G = H / Hkv;
+  scan_tiles<TREE, RW>(a, G, s_off, s_part);
+  const int total = s_off[a.n_seqs];
+  const int grid = (int)gridDim.x;
+  // neighbouring ranges on one XCD: they read the same cached rows
+  const int w = grid % kXcds == 0 ? (int)(blockIdx.x % kXcds) * (grid / kXcds) +
+                                        (int)(blockIdx.x / kXcds)
+                                  : (int)blockIdx.x;
+  const int per = max(1, (int)(((int64_t)total + grid - 1) / grid));
+  const int r0 = (int)min((int64_t)total, (int64_t)w * per);
+  const int r1 = (int)min((int64_t)total, (int64_t)(w + 1) * per);
+  if (!a.whole && threadIdx.x == 0) a.head[2 * w] = make_int4(0, 0, 0, 0);
+  if (r0 >= r1) return;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rg = wave % RW, kg = wave / RW;
+  const int lr = lane & 31, h = lane >> 5;
+
+  Unit U;
+  int t = locate<TREE, RW>(a, s_off, r0, G, U);
+  if (!a.whole && t > 0 && threadIdx.x == 0) {
+    // the range starts inside a unit; if that unit starts in the range
+    // before, this range's workgroup of the join takes it
+    const int start = r0 - t, end = start + U.ntiles;
+    if (start >= r0 - per) {
+      a.head[2 * w] = make_int4((end - 1) / per - w + 2, U.q0, U.kvh, U.row0);
+      a.head[2 * w + 1] = make_int4(min(F::R, U.rows - U.row0), 0, 0, 0);
+    }
+  }
+
+  // -- loading -------------------------------------------------------------
+  uint4 kraw[BPW][LPB], vraw[BPW][LPB];
+  float sraw = 0.0f;             // a scale (K of keys 0 .., then V) of the wavefront's blocks
+  int ids[BPW], id_first = 0, id_unit = -1;
+  const int lrow = lane / CPR, lchunk = lane % CPR;
+  auto load_ids = [&](const Unit& u, int first) {
+    const int last = (u.kend - 1) / kBs;
+#pragma unroll
+    for (int j = 0; j < BPW; ++j) {
+      ids[j] = 0;
+      if (u.kend > 0)
+        ids[j] = physical_block(a.b, a.c.num_blocks, a.seq_begin + u.seq,
+                                min((first + lane) * (KT / kBs) + wave * BPW + j, last));
+    }
+    id_first = first;
+  };
+  auto load_tile = [&](const Unit& u, int tile, bool fresh) {
+    if (fresh || tile - id_first >= 64) load_ids(u, tile);
+    int phys[BPW];     // (read by all lanes: a readlane under a branch sees stale copies)
+#pragma unroll
+    for (int j = 0; j < BPW; ++j) phys[j] = __builtin_amdgcn_readlane(ids[j], tile - id_first);
+#pragma unroll
+    for (int j = 0; j < BPW; ++j) {
+      const int64_t at = (int64_t)phys[j] * a.c.blk + u.kvh * a.c.head;
+      const char* kp = (const char*)a.c.kv[0] + at * E::kBytes;
+      const char* vp = (const char*)a.c.kv[1] + at * E::kBytes;
+#pragma unroll
+      for (int i = 0; i < LPB; ++i) {
+        const int64_t o = (int64_t)(RPL * i + lrow) * a.c.tok * E::kBytes + 16 * lchunk;
+        kraw[j][i] = load16(kp + o);
+        vraw[j][i] = load16(vp + o);
+      }
+    }
+    if constexpr (kCodes) {
+      // lanes 0 .. 16 BPW - 1 the K scales, the next as many the V scales
+      const int key = lane % (16 * BPW);
+      const bool of_v = (lane / (16 * BPW)) & 1;
+      const int64_t block = key < 16 ? phys[0] : phys[BPW - 1];
+      const float* base = of_v ? a.c.scale[1] : a.c.scale[0];
+      sraw = base[block * a.c.sblk + (key & 15) * a.c.stok + u.kvh * a.c.shead];
+    }
+  };
+  auto write_tile = [&](const Unit& u, int tile) {
+    const int key0 = tile * KT + wave * 16 * BPW;
+    const bool tail = key0 + 16 * BPW > u.kend;
+#pragma unroll
+    for (int j = 0; j < BPW; ++j)
+#pragma unroll
+      for (int i = 0; i < LPB; ++i) {
+        const int row = 16 * (wave * BPW + j) + RPL * i + lrow;    // of the tile
+        if (tail && tile * KT + row >= u.kend) vraw[j][i] = make_uint4(0, 0, 0, 0);
+        uint4 ko[OPC], vo[OPC];
+        if constexpr (kCodes) {
+          codes_to_operands<typename P::K, C>(kraw[j][i], ko);
+          codes_to_operands<typename P::V, C>(vraw[j][i], vo);
+        } else {
+          ko[0] = kraw[j][i];
+          vo[0] = vraw[j][i];
+        }
+#pragma unroll
+        for (int c = 0; c < OPC; ++c) {
+          store16(Ks + L::at(row, lchunk * OPC + c), ko[c]);
+          store16(Vs + L::at(row, lchunk * OPC + c), vo[c]);
+        }
+      }
+    if constexpr (kCodes) {
+      const int key = lane % (16 * BPW), kv = lane / (16 * BPW);
+      const int row = 16 * wave * BPW + key;
+      if (kv == 0) s_ks[row] = sraw * a.r.scale_log2;
+      if (kv == 1) s_vs[row] = tile * KT + row < u.kend ? sraw : 0.0f;
+    }
+  };
+
+  // -- a piece's state -------------------------------------------------------
+  using qv8 = typename KM::v8;
+  qv8 qf[P::QP][QSTEPS];
+  f32x16_t o[DBLK];
+  float m_run = kNegBig, l_run = 0.0f;
+  int qrow = 0, qhead = 0, lim = 0;          // this lane's row, head and last key
+  bool live = false;
+
+  auto start = [&](const Unit& u) {
+    const int idx = u.row0 + 32 * rg + lr;
+    live = idx < u.rows;
+    const int use = live ? idx : u.row0;
+    qrow = u.q0 + use / G;
+    qhead = u.kvh * G + use % G;
+    lim = TREE ? u.kend - 1 : min(u.committed + use / G, u.kend - 1);
+    const T* qp = (const T*)a.r.q + (int64_t)qrow * a.r.q_stride + (int64_t)qhead * D + 8 * h;
+#pragma unroll
+    for (int s = 0; s < QSTEPS; ++s) {
+      if constexpr (P::QP == 1) {
+        qf[0][s] = __builtin_bit_cast(qv8, load16(qp + 16 * s));
+      } else {
+        float x[8];
+        elem<float>::unpack(load16(qp + 16 * s), x);
+        elem<float>::unpack(load16(qp + 16 * s + 4), x + 4);
+#pragma unroll
+        for (int p = 0; p < P::QP; ++p) {
+          uint32_t part[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            part[i] = take_part<bf16>(x[2 * i], x[2 * i + 1], p + 1 == P::QP);
+          qf[p][s] = __builtin_bit_cast(qv8, make_uint4(part[0], part[1], part[2], part[3]));
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+    m_run = kNegBig;
+    l_run = 0.0f;
+  };
+
+  int kx[QSTEPS];
+  {
+    const int y = h ^ L::swz(lr);
+#pragma unroll
+    for (int s = 0; s < QSTEPS; ++s) kx[s] = lr * D + 8 * ((2 * s) ^ y);
+  }
+  int voff[DBLK][2];
+  {
+    const int vrow = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+    for (int b = 0; b < DBLK; ++b) {
+      const int dim = 32 * b + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      voff[b][0] = L::at(vrow, dim >> 3) + (dim & 7);
+      voff[b][1] = L::at(vrow + 8, dim >> 3) + (dim & 7);
+    }
+  }
+
+  // Bits of the 32 drafted keys from t0 on that this lane's row sees; keys
+  // before the first drafted one are committed: seen.
+  auto tree_window = [&](int t0) -> uint32_t {
+    const uint64_t* row = a.b.mask + (int64_t)qrow * a.b.mask_words;
+    if (t0 <= -32) return ~0u;
+    if (t0 < 0) return (uint32_t)(row[0] << -t0) | ((1u << -t0) - 1);
+    const int i = t0 >> 6, s = t0 & 63;
+    uint64_t v = i < a.b.mask_words ? row[i] >> s : 0;
+    if (s > 32 && i + 1 < a.b.mask_words) v |= row[i + 1] << (64 - s);
+    return (uint32_t)v;
+  };
+
+  auto compute = [&](const Unit& u, int tile) {
+    const int k0 = tile * KT + kg * KPW;           // this wavefront's first key
+    const uint16_t* kt = Ks + kg * KPW * D;
+    const uint16_t* vt = Vs + kg * KPW * D;
+    f32x16_t sv[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int s = 0; s < QSTEPS; ++s) {
+        const qv8 kf = __builtin_bit_cast(
+            qv8, *reinterpret_cast<const uint4*>(kt + 32 * kb * D + kx[s]));
+#pragma unroll
+        for (int p = P::QP - 1; p >= 0; --p)       // the small parts first
+          sv[kb] = KM::run(kf, qf[p][s], s || p + 1 < P::QP ? sv[kb] : f32x16_t{});
+      }
+    }
+    // x in log2 units; the first key that some row may not see
+    float mx = kNegBig;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const float4 ks = *reinterpret_cast<const float4*>(s_ks + kg * KPW + 32 * kb + 8 * q4 + 4 * h);
+          sv[kb][4 * q4] *= ks.x; sv[kb][4 * q4 + 1] *= ks.y;
+          sv[kb][4 * q4 + 2] *= ks.z; sv[kb][4 * q4 + 3] *= ks.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sv[kb][i] *= a.r.scale_log2;
+      }
+    }
+    const int open = TREE ? u.committed : u.committed + u.row0 / G + 1;
+    if (k0 + KPW > min(open, u.kend)) {            // the same in all lanes
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int kk = k0 + 32 * kb;
+        uint32_t win = ~0u;
+        if constexpr (TREE) win = tree_window(kk - u.committed);
+        const int d = lim - kk - 4 * h;
+        win >>= 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = 8 * (i >> 2) + (i & 3);
+          if (at > d || !((win >> at) & 1)) sv[kb][i] = -__builtin_inff();
+        }
+      }
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sv[kb][i]);
+    mx = xor32_max(mx);
+    float alpha = 1.0f;
+    if (mx > m_run + P::kLift + 8.0f) {
+      alpha = fast_exp2(m_run - (mx - P::kLift));
+      m_run = mx - P::kLift;
+    }
+    if (__ballot(alpha != 1.0f)) {                 // rare after a row's first tile
+      l_run *= alpha;
+#pragma unroll
+      for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[b][i] *= alpha;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sv[kb][i] = fast_exp2(sv[kb][i] - m_run);
+        l_run += sv[kb][i];
+      }
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const float4 vs = *reinterpret_cast<const float4*>(s_vs + kg * KPW + 32 * kb + 8 * q4 + 4 * h);
+          sv[kb][4 * q4] *= vs.x; sv[kb][4 * q4 + 1] *= vs.y;
+          sv[kb][4 * q4 + 2] *= vs.z; sv[kb][4 * q4 + 3] *= vs.w;
+        }
+      }
+      uint32_t pw[P::PP][8];
+#pragma unroll
+      for (int p = 0; p < P::PP; ++p)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float x = sv[kb][2 * i], y = sv[kb][2 * i + 1];
+          pw[p][i] = take_part<typename P::V>(x, y, p + 1 == P::PP);
+          sv[kb][2 * i] = x;
+          sv[kb][2 * i + 1] = y;
+        }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint16_t* vb = vt + (32 * kb + 16 * s) * D;
+        i16x4_t lo[DBLK], hi[DBLK];
+#pragma unroll
+        for (int b = 0; b < DBLK; ++b) {
+          lo[b] = lds_read_tr16(vb + voff[b][0]);
+          hi[b] = lds_read_tr16(vb + voff[b][1]);
+        }
+#pragma unroll
+        for (int p = P::PP - 1; p >= 0; --p) {
+          const uint32_t* pp = &pw[p][4 * s];
+          const auto pb = __builtin_bit_cast(typename VM::v8, make_uint4(pp[0], pp[1], pp[2], pp[3]));
+#pragma unroll
+          for (int b = 0; b < DBLK; ++b) {
+            const i16x8_t va = __builtin_shufflevector(lo[b], hi[b], 0, 1, 2, 3, 4, 5, 6, 7);
+            o[b] = VM::run(__builtin_bit_cast(typename VM::v8, va), pb, o[b]);
+          }
+        }
+      }
+    }
+  };
+
+  // The piece's tiles [t0, t1) again, key by key: a lane's row against every
+  // key of this wavefront that it sees, in the same dims.
+  auto careful = [&](const Unit& u, int t0, int t1) {
+    m_run = kNegBig;
+    l_run = 0.0f;
+#pragma unroll
+    for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+    const T* qp = (const T*)a.r.q + (int64_t)qrow * a.r.q_stride + (int64_t)qhead * D;
+#pragma unroll 1
+    for (int i = t0 * KPW; i < t1 * KPW; ++i) {
+      const int key = i / KPW * KT + kg * KPW + i % KPW;
+      if (key >= u.kend) continue;
+      bool sees = key <= lim;
+      if (TREE && key >= u.committed) {
+        const int tt = key - u.committed;
+        sees = sees && (tt >> 6) < a.b.mask_words &&
+               (a.b.mask[(int64_t)qrow * a.b.mask_words + (tt >> 6)] >> (tt & 63)) & 1;
+      }
+      if (!sees) continue;
+      const int64_t phys = physical_block(a.b, a.c.num_blocks, a.seq_begin + u.seq, key / kBs);
+      const int64_t at = phys * a.c.blk + (key % kBs) * a.c.tok + u.kvh * a.c.head;
+      const char* kp = (const char*)a.c.kv[0] + at * E::kBytes;
+      float x = 0.0f;
+#pragma unroll 1
+      for (int d = 0; d < D; d += E::kPer16B) {
+        float kf[E::kPer16B];
+        E::unpack(load16(kp + d * E::kBytes), kf);
+#pragma unroll
+        for (int e = 0; e < E::kPer16B; ++e) x = fmaf(elem<T>::load(qp + d + e), kf[e], x);
+      }
+      x *= a.r.scale_log2;
+      float vs = 1.0f;
+      if constexpr (kCodes) {
+        const int64_t so = phys * a.c.sblk + (key % kBs) * a.c.stok + u.kvh * a.c.shead;
+        x *= a.c.scale[0][so];
+        vs = a.c.scale[1][so];
+      }
+      const float mn = fmaxf(m_run, x), alpha = fast_exp2(m_run - mn);
+      const float p = fast_exp2(x - mn);
+      m_run = mn;
+      l_run = l_run * alpha + (h == 0 ? p : 0.0f);   // both halves hold the row
+      const char* vp = (const char*)a.c.kv[1] + (at + 4 * h) * E::kBytes;
+#pragma unroll
+      for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          float v[4];
+          const char* vq = vp + (32 * b + 8 * q4) * E::kBytes;
+          if constexpr (kCodes) {
+            code<C>::unpack4(*reinterpret_cast<const uint32_t*>(vq), v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = elem<C>::load((const C*)vq + e);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[b][4 * q4 + e] = fmaf(p * vs, v[e], o[b][4 * q4 + e] * alpha);
+        }
+    }
+  };
+
+  // Four dims of a row: to the output, or to the piece's slot.
+  auto put = [&](const Unit& u, int slot, int idx, int d, float x0, float x1, float x2, float x3) {
+    if (slot < 0) {
+      T* op = (T*)a.r.out + (int64_t)qrow * a.r.out_stride + (int64_t)qhead * D + d;
+      if constexpr (std::is_same<T, float>::value)
+        *reinterpret_cast<float4*>(op) = make_float4(x0, x1, x2, x3);
+      else
+        *reinterpret_cast<uint2*>(op) = make_uint2(Mfma32<T>::pack2(x0, x1), Mfma32<T>::pack2(x2, x3));
+    } else {
+      *reinterpret_cast<float4*>(a.acc + ((int64_t)slot * a.slot_rows + idx) * D + d) =
+          make_float4(x0, x1, x2, x3);
+    }
+  };
+  auto finish = [&](const Unit& u, int t0, int t1) {
+    float all = 0.0f;
+#pragma unroll
+    for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) all += o[b][i];
+    if (__ballot(!(fabsf(all) < __builtin_inff()))) careful(u, t0, t1);
+    const bool whole = t0 == 0 && t1 == u.ntiles;
+    const int slot = whole ? -1 : 2 * w + (t0 == 0 ? 1 : 0);
+    const int idx = 32 * rg + lr;                  // the row's place in the unit
+    l_run = xor32_sum(l_run);
+    if constexpr (KW == 1) {
+      const float inv = l_run != 0.0f ? 1.0f / l_run : 0.0f;
+      if (!live) return;
+      if (!whole && h == 0)
+        *reinterpret_cast<float2*>(a.ml + ((int64_t)slot * a.slot_rows + idx) * 2) =
+            make_float2(m_run, l_run);
+#pragma unroll
+      for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          put(u, slot, idx, 32 * b + 8 * q4 + 4 * h, o[b][4 * q4] * inv, o[b][4 * q4 + 1] * inv,
+              o[b][4 * q4 + 2] * inv, o[b][4 * q4 + 3] * inv);
+    } else {
+      constexpr int GRP = DBLK * 4 / KW;           // groups of four dims each wavefront ends with
+      float4* const xo = reinterpret_cast<float4*>(s_dyn);     // [4][DBLK * 4][64]
+      team_barrier();                              // nobody reads the tiles any more
+#pragma unroll
+      for (int b = 0; b < DBLK; ++b)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          xo[(wave * (DBLK * 4) + 4 * b + q4) * 64 + lane] =
+              make_float4(o[b][4 * q4], o[b][4 * q4 + 1], o[b][4 * q4 + 2], o[b][4 * q4 + 3]);
+      if (h == 0) s_ml[wave * 32 + lr] = make_float2(m_run, l_run);
+      team_barrier();
+      float2 ml[KW];
+      float m = kNegBig, l = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        ml[k] = s_ml[(k * RW + rg) * 32 + lr];
+        m = fmaxf(m, ml[k].x);
+      }
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        ml[k].x = fast_exp2(ml[k].x - m);
+        l += ml[k].x * ml[k].y;
+      }
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+      if (live && !whole && h == 0 && kg == 0)
+        *reinterpret_cast<float2*>(a.ml + ((int64_t)slot * a.slot_rows + idx) * 2) =
+            make_float2(m, l);
+#pragma unroll
+      for (int i = 0; i < GRP; ++i) {
+        const int grp = kg * GRP + i;
+        float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+          const float4 v = xo[((k * RW + rg) * (DBLK * 4) + grp) * 64 + lane];
+          s.x = fmaf(v.x, ml[k].x, s.x); s.y = fmaf(v.y, ml[k].x, s.y);
+          s.z = fmaf(v.z, ml[k].x, s.z); s.w = fmaf(v.w, ml[k].x, s.w);
+        }
+        if (live)
+          put(u, slot, idx, 32 * (grp >> 2) + 8 * (grp & 3) + 4 * h, s.x * inv, s.y * inv,
+              s.z * inv, s.w * inv);
+      }
+      team_barrier();                              // the next tile may be written
+    }
+  };
+
+  // -- the range ---------------------------------------------------------------
+  load_tile(U, t, true);
+  int first = t, p = r0;
+  bool fresh = true;
+  while (true) {
+    if constexpr (RW > 1) team_barrier();          // the last tile has been read
+    write_tile(U, t);
+    const bool inside = t + 1 < U.ntiles && (a.whole || p + 1 < r1);
+    const bool more = inside || p + 1 < r1;
+    Unit N = U;
+    int nt = t + 1;
+    if (more) {
+      if (!inside) {
+        N = next_unit<TREE, RW>(a, U, G);
+        nt = 0;
+      }
+      load_tile(N, nt, !inside);
+    }
+    if (fresh) start(U);
+    if constexpr (RW > 1) team_barrier();
+    else wait_lds();
+    compute(U, t);
+    fresh = !inside;
+    if (!inside) {
+      finish(U, first, t + 1);
+      first = 0;
+    }
+    if (!more) break;
+    if (!a.whole || !inside) ++p;
+    U = N;
+    t = nt;
+  }
+}
+
+// Joins the pieces of the units that span several ranges: workgroup (w, y)
+// the unit that crosses the start of range w and begins in range w - 1, its
+// rows rows_per y ...  Its pieces lie in slots 2 (w - 1) + 1, 2 w, 2 (w + 1),
+// ...  D / 4 lanes per row, `rows_per` rows at a time, the rest of the
+// workgroup the row's other pieces.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(TileArgs a, int rows_per) {
+  constexpr int LPR = D / 4, TEAMS = 256 / LPR;
+  __shared__ float2 s_ml[TEAMS];
+  __shared__ float4 s_o[TEAMS][LPR];
+  const int w = blockIdx.x + 1;
+  const int4 hd = a.head[2 * w];
+  if (hd.x == 0) return;
+  const int nrows = a.head[2 * w + 1].x;
+  const int team = threadIdx.x / LPR, d = 4 * (threadIdx.x % LPR);
+  const int parts = TEAMS / rows_per;          // pieces taken side by side
+  const int row = (int)blockIdx.y * rows_per + team / parts;
+  const bool on = row < nrows;
+  float m = kNegBig, l = 0.0f, o[4] = {};
+  if (on) {
+    for (int i = team % parts; i < hd.x; i += parts) {
+      const int64_t slot = i == 0 ? 2 * (w - 1) + 1 : 2 * (w - 1 + i);
+      const float2 ml = *reinterpret_cast<const float2*>(a.ml + (slot * a.slot_rows + row) * 2);
+      const float4 v = *reinterpret_cast<const float4*>(a.acc + (slot * a.slot_rows + row) * D + d);
+      const float mn = fmaxf(m, ml.x), f0 = fast_exp2(m - mn), f1 = ml.y * fast_exp2(ml.x - mn);
+      m = mn;
+      l = l * f0 + f1;
+      o[0] = o[0] * f0 + v.x * f1; o[1] = o[1] * f0 + v.y * f1;
+      o[2] = o[2] * f0 + v.z * f1; o[3] = o[3] * f0 + v.w * f1;
+    }
+  }
+  if (parts > 1) {
+    if (d == 0) s_ml[team] = make_float2(m, l);
+    s_o[team][d / 4] = make_float4(o[0], o[1], o[2], o[3]);
+    __syncthreads();
+    if (team % parts != 0 || !on) return;
+    for (int k = 1; k < parts; ++k) {
+      const float2 ml = s_ml[team + k];
+      const float4 v = s_o[team + k][d / 4];
+      const float mn = fmaxf(m, ml.x), f0 = fast_exp2(m - mn), f1 = fast_exp2(ml.x - mn);
+      m = mn;
+      l = l * f0 + ml.y * f1;
+      o[0] = o[0] * f0 + v.x * f1; o[1] = o[1] * f0 + v.y * f1;
+      o[2] = o[2] * f0 + v.z * f1; o[3] = o[3] * f0 + v.w * f1;
+    }
+  }
+  if (!on) return;
+  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+  const int g = a.r.num_heads / a.r.num_kv_heads;
+  const int idx = hd.w + row;
+  T* op = (T*)a.r.out + (int64_t)(hd.y + idx / g) * a.r.out_stride +
+          (int64_t)(hd.z * g + idx % g) * D + d;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) elem<T>::store(op + i, o[i] * inv);
+}
+
+// ---------------------------------------------------------------------------
+// Launch.
+// ---------------------------------------------------------------------------
+template <typename T, typename C, int D, int RW, bool TREE>
+int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
+  using F = TileCfg<RW>;
+  TileArgs t{};
+  t.b = a.b; t.c = a.c; t.r = a.r;
+  t.seq_begin = p.seq_begin; t.n_seqs = p.n_seqs; t.max_q = p.max_q;
+  t.whole = p.whole;
+  t.slot_rows = p.slot_rows;
+  t.head = reinterpret_cast<int4*>(ws);
+  t.ml = reinterpret_cast<float*>(ws + p.head_bytes);
+  t.acc = reinterpret_cast<float*>(ws + p.head_bytes + p.ml_bytes);
+  const size_t lds = (size_t)F::KT * D * 4 + F::KT * 8 + 128 * 8 + (size_t)(p.n_seqs + 1) * 4;
+  attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, kTileThreads, lds, a.stream>>>(t);
+  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.whole || p.grid < 2)
+    return rc;
+  constexpr int TEAMS = 256 / (D / 4);
+  int rows_per = 1;
+  while (rows_per < TEAMS && rows_per * 2 < p.slot_rows) rows_per *= 2;
+  attn_join_kernel<T, D><<<dim3((unsigned)p.grid - 1, (unsigned)((p.slot_rows + rows_per - 1) / rows_per)),
+                           256, 0, a.stream>>>(t, rows_per);
+  return check_launch("attn_join_kernel");
+}
+
+template <typename T, typename C, int D>
+int launch_tiles_d(const Call& a, const TilePlan& p, char* ws) {
+  if (a.tree) {
+    if (p.rw == 1) return launch_tile_kernel<T, C, D, 1, true>(a, p, ws);
+    if (p.rw == 2) return launch_tile_kernel<T, C, D, 2, true>(a, p, ws);
+    return launch_tile_kernel<T, C, D, 4, true>(a, p, ws);
+  }
+  if constexpr (cached<C>::kCodes) {
+    if (p.rw == 1) return launch_tile_kernel<T, C, D, 1, false>(a, p, ws);
+    if (p.rw == 2) return launch_tile_kernel<T, C, D, 2, false>(a, p, ws);
+    return launch_tile_kernel<T, C, D, 4, false>(a, p, ws);
+  }
+  return LV_ERR_UNSUPPORTED;
+}
+
+template <typename T>
+int launch_tiles(const Call& a, const TilePlan& p, char* ws) {
+  if (a.code == LV_INT8)
+    return a.d == 64 ? launch_tiles_d<T, int8_code, 64>(a, p, ws)
+                     : launch_tiles_d<T, int8_code, 128>(a, p, ws);
+  if (a.code == LV_E4M3)
+    return a.d == 64 ? launch_tiles_d<T, e4m3_code, 64>(a, p, ws)
+                     : launch_tiles_d<T, e4m3_code, 128>(a, p, ws);
+  if constexpr (!std::is_same<T, float>::value)
+    return a.d == 64 ? launch_tiles_d<T, T, 64>(a, p, ws) : launch_tiles_d<T, T, 128>(a, p, ws);
+  return LV_ERR_UNSUPPORTED;
+}
+
+}  // namespace lv

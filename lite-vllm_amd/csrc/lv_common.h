@@ -215,6 +215,9 @@ int read_errors_attention(uint32_t* bits, bool clear);
 int read_errors_fused(uint32_t* bits, bool clear);
 int read_errors_quant(uint32_t* bits, bool clear);
 int read_errors_tree(uint32_t* bits, bool clear);
+int read_errors_tiles_bf16(uint32_t* bits, bool clear);
+int read_errors_tiles_f16(uint32_t* bits, bool clear);
+int read_errors_tiles_f32(uint32_t* bits, bool clear);
 
 // Checks a cache description on the host (kv_quant.hip).
 int check_quant_cache(const char* who, const lv_quant_cache* cache);

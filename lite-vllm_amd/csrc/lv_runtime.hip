@@ -43,7 +43,8 @@ extern "C" int lv_device_errors(uint32_t* flags_out, int32_t clear) {
   }
   int (*const readers[])(uint32_t*, bool) = {read_errors_scatter, read_errors_attention,
                                              read_errors_fused, read_errors_quant,
-                                             read_errors_tree};
+                                             read_errors_tree, read_errors_tiles_bf16,
+                                             read_errors_tiles_f16, read_errors_tiles_f32};
   uint32_t all = 0;
   for (auto rd : readers) {
     uint32_t v = 0;
