@@ -19,8 +19,10 @@
 #include <ATen/autocast_mode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -47,6 +49,14 @@ struct Api {
   decltype(&lv_linear_one_round) linear_one_round;
   decltype(&lv_linear) linear;
   decltype(&lv_linear_f32) linear_f32;
+  decltype(&lv_kv_scatter_quant) kv_scatter_quant;
+  decltype(&lv_kv_gather_quant) kv_gather_quant;
+  decltype(&lv_qk_norm_rope_cache_quant) qk_norm_rope_cache_quant;
+  decltype(&lv_paged_attention_quant_workspace_size) attention_quant_ws;
+  decltype(&lv_paged_attention_quant) attention_quant;
+  decltype(&lv_tree_attention_workspace_size) tree_ws;
+  decltype(&lv_tree_attention) tree;
+  decltype(&lv_tree_attention_quant) tree_quant;
 };
 Api api{};
 
@@ -55,7 +65,10 @@ constexpr const char* kNames[] = {
     "lv_paged_attention_split_workspace_size", "lv_paged_attention",
     "lv_paged_attention_prefix_workspace_size", "lv_paged_attention_prefix",
     "lv_sample_workspace_size", "lv_sample", "lv_add_rms_norm", "lv_qk_norm_rope_cache",
-    "lv_silu_mul", "lv_linear_one_round", "lv_linear", "lv_linear_f32"};
+    "lv_silu_mul", "lv_linear_one_round", "lv_linear", "lv_linear_f32", "lv_kv_scatter_quant",
+    "lv_kv_gather_quant", "lv_qk_norm_rope_cache_quant", "lv_paged_attention_quant_workspace_size",
+    "lv_paged_attention_quant", "lv_tree_attention_workspace_size", "lv_tree_attention",
+    "lv_tree_attention_quant"};
 constexpr size_t kNumNames = sizeof(kNames) / sizeof(kNames[0]);
 static_assert(sizeof(Api) == kNumNames * sizeof(void*), "one pointer per name");
 
@@ -451,6 +464,246 @@ FAST(linear_f32, 3) {
   return done(rc, "lv_linear_f32", &out);
 }
 
+// An 8-bit cache: QuantKV(key, value, key_scale, value_scale).
+struct QuantArg {
+  const at::Tensor *k = nullptr, *v = nullptr, *ks = nullptr, *vs = nullptr;
+  lv_quant_cache c{};
+
+  // Reads argument i of A; false if it is not of the plain form.
+  bool read(const Args& A, int i) {
+    if (!PyTuple_Check(A.a[i]) || PyTuple_GET_SIZE(A.a[i]) != 4) return false;
+    Args P{((PyTupleObject*)A.a[i])->ob_item};
+    k = P.tensor(0); v = P.tensor(1); ks = P.tensor(2); vs = P.tensor(3);
+    if (!P.ok || !k->is_cuda() || k->dim() != 4 || ks->dim() != 3 || k->sizes() != v->sizes() ||
+        k->strides() != v->strides() || ks->sizes() != vs->sizes() ||
+        ks->strides() != vs->strides() || k->sizes().slice(0, 3) != ks->sizes() ||
+        k->stride(3) != 1 || v->scalar_type() != k->scalar_type() ||
+        ks->scalar_type() != at::kFloat || vs->scalar_type() != at::kFloat)
+      return false;
+    if (k->scalar_type() == at::kChar) c.code = LV_INT8;
+    else if (k->scalar_type() == at::kFloat8_e4m3fn) c.code = LV_E4M3;
+    else return false;
+    for (const at::Tensor* t : {k, v, ks, vs})
+      if (!on(t, k->device())) return false;
+    for (int d = 1; d < 4; ++d)
+      if (k->size(d) > INT32_MAX) return false;
+    c.key_dev = k->data_ptr(); c.value_dev = v->data_ptr();
+    c.key_scale_dev = (float*)ks->data_ptr(); c.value_scale_dev = (float*)vs->data_ptr();
+    c.num_blocks = k->size(0); c.block_size = k->size(1);
+    c.num_kv_heads = k->size(2); c.head_dim = k->size(3);
+    c.stride_block = k->stride(0); c.stride_token = k->stride(1); c.stride_head = k->stride(2);
+    c.scale_stride_block = ks->stride(0); c.scale_stride_token = ks->stride(1);
+    c.scale_stride_head = ks->stride(2);
+    return true;
+  }
+};
+
+// Whether `dev` is the current device (else the wrappers change to it).
+bool is_current(const at::Device& dev) { return c10::hip::current_device() == dev.index(); }
+
+// (key, value, cache, slot_mapping) -> True
+FAST(kv_scatter_quant, 4) {
+  const at::Tensor *k = A.tensor(0), *v = A.tensor(1), *slots = A.tensor(3);
+  QuantArg q;
+  lv_dtype dt;
+  if (!A.ok || !q.read(A, 2) || !dtype_of(*k, dt)) NOT_PLAIN();
+  const at::Device dev = q.k->device();
+  const int64_t T = slots->numel(), hkv = q.c.num_kv_heads, d = q.c.head_dim;
+  if (!on(k, dev) || !on(v, dev) || !on(slots, dev) || T == 0 || !is_current(dev) ||
+      !is_array(*slots, at::kLong, 1) || !is_heads(*k, hkv, d) || !is_heads(*v, hkv, d) ||
+      k->size(0) != T || v->size(0) != T || v->scalar_type() != k->scalar_type())
+    NOT_PLAIN();
+  void* st = stream_of(dev);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.kv_scatter_quant(ptr(k), k->stride(0), ptr(v), v->stride(0), &q.c,
+                            (const int64_t*)ptr(slots), T, dt, st);
+  Py_END_ALLOW_THREADS
+  return done(rc, "lv_kv_scatter_quant", nullptr);
+}
+
+// (cache, slots, dtype, out) -> (key, value)
+FAST(kv_gather_quant, 4) {
+  const at::Tensor* slots = A.tensor(1);
+  QuantArg q;
+  lv_dtype dt;
+  if (!A.ok || !q.read(A, 0) || !THPDtype_Check(A.a[2]) || A.a[3] != Py_None) NOT_PLAIN();
+  const at::ScalarType type = ((THPDtype*)A.a[2])->scalar_type;
+  const at::Device dev = q.k->device();
+  const int64_t T = slots->numel();
+  if (!on(slots, dev) || T == 0 || !is_current(dev) || !is_array(*slots, at::kLong, 1) ||
+      (type != at::kFloat && type != at::kHalf && type != at::kBFloat16))
+    NOT_PLAIN();
+  const at::TensorOptions opt = at::TensorOptions().dtype(type).device(dev);
+  const at::Tensor key = at::empty({T, q.c.num_kv_heads, q.c.head_dim}, opt),
+                   value = at::empty({T, q.c.num_kv_heads, q.c.head_dim}, opt);
+  dtype_of(key, dt);
+  void* st = stream_of(dev);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.kv_gather_quant(&q.c, (const int64_t*)ptr(slots), T, key.data_ptr(), key.stride(0),
+                           value.data_ptr(), value.stride(0), dt, st);
+  Py_END_ALLOW_THREADS
+  PyObject* k = done(rc, "lv_kv_gather_quant", &key);
+  if (!k) return nullptr;
+  return Py_BuildValue("(NN)", k, THPVariable_Wrap(value));
+}
+
+// (qkv, num_heads, num_kv_heads, head_dim, cos, sin, positions, slot_mapping,
+//  cache, q_norm_weight, k_norm_weight, eps, q_out) -> q_out
+FAST(qk_norm_rope_cache_quant, 13) {
+  const at::Tensor *qkv = A.tensor(0), *cs = A.tensor(4), *sn = A.tensor(5), *pos = A.tensor(6),
+                   *slots = A.tensor(7), *qw = A.maybe(9), *kw = A.maybe(10), *given = A.maybe(12);
+  const int64_t H = A.integer(1), Hkv = A.integer(2), D = A.integer(3);
+  const double eps = A.number(11);
+  QuantArg q;
+  lv_dtype dt;
+  if (!A.ok || H < 1 || !q.read(A, 8) || !dtype_of(*qkv, dt) || q.c.num_kv_heads != Hkv ||
+      q.c.head_dim != D)
+    NOT_PLAIN();
+  const at::Device dev = q.k->device();
+  const at::ScalarType type = qkv->scalar_type();
+  for (const at::Tensor* t : {qkv, cs, sn, pos, slots, qw, kw, given})
+    if (!on(t, dev)) NOT_PLAIN();
+  if (!is_current(dev) || !is_rows(*qkv, (H + 2 * Hkv) * D, type) ||
+      !is_array(*pos, at::kLong, 1) || !is_array(*slots, at::kLong, 1))
+    NOT_PLAIN();
+  const int64_t T = qkv->size(0);
+  if (T == 0 || pos->size(0) != T || slots->size(0) != T) NOT_PLAIN();
+  for (const at::Tensor* t : {cs, sn})
+    if (!is_array(*t, type, 2) || t->size(1) != D / 2) NOT_PLAIN();
+  if (sn->size(0) != cs->size(0)) NOT_PLAIN();
+  for (const at::Tensor* t : {qw, kw})
+    if (t && (!is_array(*t, type, 1) || t->size(0) != D)) NOT_PLAIN();
+  if (given && (!is_heads(*given, H, D) || given->size(0) != T || given->scalar_type() != type))
+    NOT_PLAIN();
+  const at::Tensor out = given ? *given : empty({T, H, D}, *qkv);
+  void* st = stream_of(dev);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.qk_norm_rope_cache_quant(ptr(qkv), qkv->stride(0), ptr(qw), ptr(kw), ptr(cs), ptr(sn),
+                                    cs->size(0), (const int64_t*)ptr(pos),
+                                    (const int64_t*)ptr(slots), out.data_ptr(), out.stride(0),
+                                    &q.c, T, H, (float)eps, dt, st);
+  Py_END_ALLOW_THREADS
+  return done(rc, "lv_qk_norm_rope_cache_quant", &out);
+}
+
+// The batch of an attention call: query, block_tables, context_lens,
+// cu_seqlens (or none) and out (or none) on `dev`.
+bool is_batch(const at::Device& dev, const at::Tensor* q, const at::Tensor* bt,
+              const at::Tensor* ctx, const at::Tensor* cu, const at::Tensor* given) {
+  if (!is_current(dev) || !on(q, dev) || !on(bt, dev) || !on(ctx, dev) || !on(cu, dev) ||
+      !on(given, dev) || q->dim() != 3 || !is_heads(*q, q->size(1), q->size(2)) ||
+      !is_array(*bt, at::kInt, 2) || !is_array(*ctx, at::kInt, 1))
+    return false;
+  const int64_t T = q->size(0), B = bt->size(0);
+  return T > 0 && B > 0 && ctx->size(0) == B && T <= INT32_MAX && bt->size(1) <= INT32_MAX &&
+         (cu ? is_array(*cu, at::kInt, 1) && cu->size(0) == B + 1 : T == B) &&
+         (!given || (is_heads(*given, q->size(1), q->size(2)) && given->size(0) == T &&
+                     given->scalar_type() == q->scalar_type()));
+}
+
+// (query, cache, block_tables, context_lens, scale, cu_seqlens, num_decodes,
+//  max_query_len, out, workspace) -> out
+FAST(paged_attention_quant, 10) {
+  const at::Tensor *q = A.tensor(0), *bt = A.tensor(2), *ctx = A.tensor(3), *cu = A.maybe(5),
+                   *given = A.maybe(8), *ws = A.maybe(9);
+  const double scale = A.number(4);
+  const int64_t max_q = A.integer(7);
+  QuantArg c;
+  lv_dtype dt;
+  if (!A.ok || !c.read(A, 1) || !dtype_of(*q, dt)) NOT_PLAIN();
+  const at::Device dev = c.k->device();
+  if (!is_batch(dev, q, bt, ctx, cu, given) || q->size(2) != c.c.head_dim || !on(ws, dev))
+    NOT_PLAIN();
+  const int64_t T = q->size(0), H = q->size(1), B = bt->size(0), max_blocks = bt->size(1);
+  int64_t nd = cu ? 0 : B;
+  if (A.a[6] != Py_None) nd = A.integer(6);
+  if (!A.ok || nd < 0 || nd > B) NOT_PLAIN();
+  const size_t bytes = api.attention_quant_ws(B, nd, T, max_q, H, c.c.num_kv_heads, c.c.head_dim,
+                                              max_blocks, dt);
+  if (ws && !is_scratch(*ws, bytes)) NOT_PLAIN();
+  void* st = stream_of(dev);
+  if (!ws && bytes > 0 && !(ws = scratch(dev, st, bytes, kind_attn))) NOT_PLAIN();
+  const at::Tensor ws_held = ws ? *ws : at::Tensor();
+  const at::Tensor out = given ? *given : empty(q->sizes(), *q);
+  void* wp = ptr(ws);
+  const size_t wn = ws ? ws->numel() : 0;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = api.attention_quant(ptr(q), q->stride(0), &c.c, (const int32_t*)ptr(bt), max_blocks,
+                           (const int32_t*)ptr(cu), (const int32_t*)ptr(ctx), B, nd, T, max_q, H,
+                           (float)scale, out.data_ptr(), out.stride(0), wp, wn, dt, st);
+  Py_END_ALLOW_THREADS
+  return done(rc, "lv_paged_attention_quant", &out);
+}
+
+// Common to the two below: arguments from `at` on are block_tables,
+// context_lens, cu_seqlens, tree_mask, scale, max_query_len, out, workspace.
+// `c` is the 8-bit cache, or null: then the caches of query's type kc, vc.
+PyObject* tree_call(Args& A, int at, const QuantArg* c, const at::Tensor* kc,
+                    const at::Tensor* vc) {
+  const at::Tensor *q = A.tensor(0), *bt = A.tensor(at), *ctx = A.tensor(at + 1),
+                   *cu = A.tensor(at + 2), *mask = A.tensor(at + 3), *given = A.maybe(at + 6),
+                   *ws = A.maybe(at + 7);
+  const double scale = A.number(at + 4);
+  const int64_t max_q = A.integer(at + 5);
+  lv_dtype dt;
+  if (!A.ok || !dtype_of(*q, dt)) NOT_PLAIN();
+  const at::Device dev = c ? c->k->device() : kc->device();
+  if (!is_batch(dev, q, bt, ctx, cu, given) || !on(ws, dev) || !on(mask, dev) ||
+      !is_array(*mask, at::kLong, 2) || mask->size(0) != q->size(0) || mask->size(1) < 1 ||
+      mask->size(1) > INT32_MAX / 64 || mask->size(1) * 64 < max_q)
+    NOT_PLAIN();
+  const int64_t T = q->size(0), H = q->size(1), D = q->size(2), B = bt->size(0),
+                max_blocks = bt->size(1);
+  if (c ? c->c.head_dim != D
+        : !on(kc, dev) || !on(vc, dev) || !is_cache(*kc) || !is_cache(*vc) ||
+              kc->sizes() != vc->sizes() || kc->size(3) != D ||
+              kc->scalar_type() != q->scalar_type() || vc->scalar_type() != q->scalar_type())
+    NOT_PLAIN();
+  const int64_t hkv = c ? c->c.num_kv_heads : kc->size(2);
+  const size_t bytes = api.tree_ws(B, T, max_q, H, hkv, D, max_blocks, dt);
+  if (ws && !is_scratch(*ws, bytes)) NOT_PLAIN();
+  void* st = stream_of(dev);
+  if (!ws && bytes > 0 && !(ws = scratch(dev, st, bytes, kind_attn))) NOT_PLAIN();
+  const at::Tensor ws_held = ws ? *ws : at::Tensor();
+  const at::Tensor out = given ? *given : empty(q->sizes(), *q);
+  void* wp = ptr(ws);
+  const size_t wn = ws ? ws->numel() : 0;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  if (c)
+    rc = api.tree_quant(ptr(q), q->stride(0), &c->c, (const int32_t*)ptr(bt), max_blocks,
+                        (const int32_t*)ptr(cu), (const int32_t*)ptr(ctx),
+                        (const uint64_t*)ptr(mask), mask->size(1), B, T, max_q, H, (float)scale,
+                        out.data_ptr(), out.stride(0), wp, wn, dt, st);
+  else
+    rc = api.tree(ptr(q), q->stride(0), ptr(kc), ptr(vc), kc->size(0), (const int32_t*)ptr(bt),
+                  max_blocks, (const int32_t*)ptr(cu), (const int32_t*)ptr(ctx),
+                  (const uint64_t*)ptr(mask), mask->size(1), B, T, max_q, H, hkv, D, kc->size(1),
+                  (float)scale, out.data_ptr(), out.stride(0), wp, wn, dt, st);
+  Py_END_ALLOW_THREADS
+  return done(rc, c ? "lv_tree_attention_quant" : "lv_tree_attention", &out);
+}
+
+// (query, key_cache, value_cache, block_tables, context_lens, cu_seqlens,
+//  tree_mask, scale, max_query_len, out, workspace) -> out
+FAST(tree_attention, 11) {
+  const at::Tensor *kc = A.tensor(1), *vc = A.tensor(2);
+  if (!A.ok || !kc->is_cuda()) NOT_PLAIN();
+  return tree_call(A, 3, nullptr, kc, vc);
+}
+
+// (query, cache, block_tables, context_lens, cu_seqlens, tree_mask, scale,
+//  max_query_len, out, workspace) -> out
+FAST(tree_attention_quant, 10) {
+  QuantArg c;
+  if (!c.read(A, 1)) NOT_PLAIN();
+  return tree_call(A, 2, &c, nullptr, nullptr);
+}
+
 // No tangent of forward-mode differentiation, and nothing between the tensor
 // and the values in its storage: no transform's wrapper, lazy conjugate or
 // negation.
@@ -550,6 +803,12 @@ PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, nullptr},
                          METHOD(linear),
                          METHOD(linear_f32),
                          METHOD(layer_linear),
+                         METHOD(kv_scatter_quant),
+                         METHOD(kv_gather_quant),
+                         METHOD(qk_norm_rope_cache_quant),
+                         METHOD(paged_attention_quant),
+                         METHOD(tree_attention),
+                         METHOD(tree_attention_quant),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 

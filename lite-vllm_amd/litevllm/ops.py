@@ -889,6 +889,8 @@ def kv_scatter_quant(key: torch.Tensor, value: torch.Tensor, cache: QuantKV,
 
     Reference: litevllm/layers/attention.py:17-33 and 79-84.
     """
+    if (_native_module or _native()).kv_scatter_quant(key, value, cache, slot_mapping):
+        return
     c = _quant_cache(cache)
     dev = cache.key.device
     for n, t in (("key", key), ("value", value), ("slot_mapping", slot_mapping)):
@@ -901,8 +903,10 @@ def kv_scatter_quant(key: torch.Tensor, value: torch.Tensor, cache: QuantKV,
         _check_heads(n, t, (T, c.num_kv_heads, c.head_dim))
     if T == 0:
         return
-    rc = _hip.load().lv_kv_scatter_quant(_ptr(key), key.stride(0), _ptr(value), value.stride(0), c,
-                                         _ptr(slot_mapping), T, _dtype_code(key), _stream(dev))
+    with torch.cuda.device(dev):
+        rc = _hip.load().lv_kv_scatter_quant(_ptr(key), key.stride(0), _ptr(value), value.stride(0),
+                                             c, _ptr(slot_mapping), T, _dtype_code(key),
+                                             _stream(dev))
     _hip.check(rc, "lv_kv_scatter_quant")
 
 
@@ -911,6 +915,9 @@ def kv_gather_quant(cache: QuantKV, slots: torch.Tensor, dtype: torch.dtype,
                     ) -> tuple[torch.Tensor, torch.Tensor]:
     """(key, value) rows [T, Hkv, D] of an 8-bit cache at the given slots, as
     values of `dtype`; rows of zeros at negative slots."""
+    done = (_native_module or _native()).kv_gather_quant(cache, slots, dtype, out)
+    if done is not None:
+        return done
     c = _quant_cache(cache)
     dev = cache.key.device
     _require_device("slots", slots, dev)
@@ -926,8 +933,9 @@ def kv_gather_quant(cache: QuantKV, slots: torch.Tensor, dtype: torch.dtype,
     code = _dtype_code(out[0])
     if shape[0] == 0:
         return out
-    rc = _hip.load().lv_kv_gather_quant(c, _ptr(slots), shape[0], _ptr(out[0]), out[0].stride(0),
-                                        _ptr(out[1]), out[1].stride(0), code, _stream(dev))
+    with torch.cuda.device(dev):
+        rc = _hip.load().lv_kv_gather_quant(c, _ptr(slots), shape[0], _ptr(out[0]), out[0].stride(0),
+                                            _ptr(out[1]), out[1].stride(0), code, _stream(dev))
     _hip.check(rc, "lv_kv_gather_quant")
     return out
 
@@ -944,6 +952,11 @@ def qk_norm_rope_cache_quant(qkv: torch.Tensor, num_heads: int, num_kv_heads: in
     Reference: models/qwen3.py:75-84, layers/rotary_emb.py:92-117,
     layers/attention.py:79-84.
     """
+    done = (_native_module or _native()).qk_norm_rope_cache_quant(
+        qkv, num_heads, num_kv_heads, head_dim, cos_cache, sin_cache, positions, slot_mapping,
+        cache, q_norm_weight, k_norm_weight, eps, q_out)
+    if done is not None:
+        return done
     c = _quant_cache(cache)
     dev = cache.key.device
     for n, t in (("qkv", qkv), ("cos_cache", cos_cache), ("sin_cache", sin_cache),
@@ -977,10 +990,11 @@ def qk_norm_rope_cache_quant(qkv: torch.Tensor, num_heads: int, num_kv_heads: in
     code = _dtype_code(qkv)
     if T == 0:
         return q_out
-    rc = _hip.load().lv_qk_norm_rope_cache_quant(
-        _ptr(qkv), qkv.stride(0), _ptr(q_norm_weight), _ptr(k_norm_weight), _ptr(cos_cache),
-        _ptr(sin_cache), cos_cache.shape[0], _ptr(positions), _ptr(slot_mapping), _ptr(q_out),
-        q_out.stride(0), c, T, H, float(eps), code, _stream(dev))
+    with torch.cuda.device(dev):
+        rc = _hip.load().lv_qk_norm_rope_cache_quant(
+            _ptr(qkv), qkv.stride(0), _ptr(q_norm_weight), _ptr(k_norm_weight), _ptr(cos_cache),
+            _ptr(sin_cache), cos_cache.shape[0], _ptr(positions), _ptr(slot_mapping), _ptr(q_out),
+            q_out.stride(0), c, T, H, float(eps), code, _stream(dev))
     _hip.check(rc, "lv_qk_norm_rope_cache_quant")
     return q_out
 
@@ -1033,6 +1047,11 @@ def paged_attention_quant(query: torch.Tensor, cache: QuantKV, block_tables: tor
 
     Reference: litevllm/layers/attention.py:91-151.
     """
+    done = (_native_module or _native()).paged_attention_quant(
+        query, cache, block_tables, context_lens, scale, cu_seqlens, num_decodes, max_query_len,
+        out, workspace)
+    if done is not None:
+        return done
     c = _quant_cache(cache)
     dev = cache.key.device
     out = _attention_args(query, dev, block_tables, context_lens, cu_seqlens, out)
@@ -1046,13 +1065,14 @@ def paged_attention_quant(query: torch.Tensor, cache: QuantKV, block_tables: tor
     if B == 0 or T == 0:
         return out
     lib = _hip.load()
-    need = lib.lv_paged_attention_quant_workspace_size(B, num_decodes, T, max_query_len, H,
-                                                       c.num_kv_heads, D, max_blocks, dt)
-    ws = _given_workspace(workspace, need, dev)
-    rc = lib.lv_paged_attention_quant(
-        _ptr(query), query.stride(0), c, _ptr(block_tables), max_blocks, _ptr(cu_seqlens),
-        _ptr(context_lens), B, num_decodes, T, max_query_len, H, float(scale), _ptr(out),
-        out.stride(0), _ptr(ws), 0 if ws is None else ws.numel(), dt, _stream(dev))
+    with torch.cuda.device(dev):
+        need = lib.lv_paged_attention_quant_workspace_size(B, num_decodes, T, max_query_len, H,
+                                                           c.num_kv_heads, D, max_blocks, dt)
+        ws = _given_workspace(workspace, need, dev)
+        rc = lib.lv_paged_attention_quant(
+            _ptr(query), query.stride(0), c, _ptr(block_tables), max_blocks, _ptr(cu_seqlens),
+            _ptr(context_lens), B, num_decodes, T, max_query_len, H, float(scale), _ptr(out),
+            out.stride(0), _ptr(ws), 0 if ws is None else ws.numel(), dt, _stream(dev))
     _hip.check(rc, "lv_paged_attention_quant")
     return out
 
@@ -1087,8 +1107,9 @@ def tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor, max_query_len: in
     mask = torch.zeros((T, words), dtype=torch.int64, device=dev)
     if T == 0 or B <= 0:
         return mask
-    rc = _hip.load().lv_tree_mask(_ptr(parents), _ptr(cu_seqlens), B, T, _ptr(mask), words,
-                                  _stream(dev))
+    with torch.cuda.device(dev):
+        rc = _hip.load().lv_tree_mask(_ptr(parents), _ptr(cu_seqlens), B, T, _ptr(mask), words,
+                                      _stream(dev))
     _hip.check(rc, "lv_tree_mask")
     return mask
 
@@ -1120,6 +1141,11 @@ def tree_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: to
     The reference decodes one token per sequence and step
     (litevllm/layers/attention.py:91-139).
     """
+    done = (_native_module or _native()).tree_attention(
+        query, key_cache, value_cache, block_tables, context_lens, cu_seqlens, tree_mask, scale,
+        max_query_len, out, workspace)
+    if done is not None:
+        return done
     dev = key_cache.device
     for n, t in (("key_cache", key_cache), ("value_cache", value_cache)):
         _require_device(n, t, dev)
@@ -1137,13 +1163,14 @@ def tree_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: to
     if B == 0 or T == 0:
         return out
     lib = _hip.load()
-    need = lib.lv_tree_attention_workspace_size(B, T, max_query_len, H, hkv, D, max_blocks, dt)
-    ws = _given_workspace(workspace, need, dev)
-    rc = lib.lv_tree_attention(
-        _ptr(query), query.stride(0), _ptr(key_cache), _ptr(value_cache), n_blocks,
-        _ptr(block_tables), max_blocks, _ptr(cu_seqlens), _ptr(context_lens), _ptr(tree_mask),
-        words, B, T, max_query_len, H, hkv, D, bs, float(scale), _ptr(out), out.stride(0), _ptr(ws),
-        0 if ws is None else ws.numel(), dt, _stream(dev))
+    with torch.cuda.device(dev):
+        need = lib.lv_tree_attention_workspace_size(B, T, max_query_len, H, hkv, D, max_blocks, dt)
+        ws = _given_workspace(workspace, need, dev)
+        rc = lib.lv_tree_attention(
+            _ptr(query), query.stride(0), _ptr(key_cache), _ptr(value_cache), n_blocks,
+            _ptr(block_tables), max_blocks, _ptr(cu_seqlens), _ptr(context_lens), _ptr(tree_mask),
+            words, B, T, max_query_len, H, hkv, D, bs, float(scale), _ptr(out), out.stride(0), _ptr(ws),
+            0 if ws is None else ws.numel(), dt, _stream(dev))
     _hip.check(rc, "lv_tree_attention")
     return out
 
@@ -1157,6 +1184,11 @@ def tree_attention_quant(query: torch.Tensor, cache: QuantKV, block_tables: torc
 
     Reference: litevllm/layers/attention.py:91-139.
     """
+    done = (_native_module or _native()).tree_attention_quant(
+        query, cache, block_tables, context_lens, cu_seqlens, tree_mask, scale, max_query_len,
+        out, workspace)
+    if done is not None:
+        return done
     c = _quant_cache(cache)
     dev = cache.key.device
     out = _attention_args(query, dev, block_tables, context_lens, cu_seqlens, out)
@@ -1169,13 +1201,14 @@ def tree_attention_quant(query: torch.Tensor, cache: QuantKV, block_tables: torc
     if B == 0 or T == 0:
         return out
     lib = _hip.load()
-    need = lib.lv_tree_attention_workspace_size(B, T, max_query_len, H, c.num_kv_heads, D,
-                                                max_blocks, dt)
-    ws = _given_workspace(workspace, need, dev)
-    rc = lib.lv_tree_attention_quant(
-        _ptr(query), query.stride(0), c, _ptr(block_tables), max_blocks, _ptr(cu_seqlens),
-        _ptr(context_lens), _ptr(tree_mask), words, B, T, max_query_len, H, float(scale),
-        _ptr(out), out.stride(0), _ptr(ws), 0 if ws is None else ws.numel(), dt, _stream(dev))
+    with torch.cuda.device(dev):
+        need = lib.lv_tree_attention_workspace_size(B, T, max_query_len, H, c.num_kv_heads, D,
+                                                    max_blocks, dt)
+        ws = _given_workspace(workspace, need, dev)
+        rc = lib.lv_tree_attention_quant(
+            _ptr(query), query.stride(0), c, _ptr(block_tables), max_blocks, _ptr(cu_seqlens),
+            _ptr(context_lens), _ptr(tree_mask), words, B, T, max_query_len, H, float(scale),
+            _ptr(out), out.stride(0), _ptr(ws), 0 if ws is None else ws.numel(), dt, _stream(dev))
     _hip.check(rc, "lv_tree_attention_quant")
     return out
 
