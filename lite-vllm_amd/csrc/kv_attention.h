@@ -80,11 +80,12 @@ struct Call {
 };
 
 // The sequences [seq_begin, seq_begin + n_seqs) of a call, max_q rows each at
-// most, on the tile kernel: how it is launched and laid out in the workspace.
+// most: their kernel, its launch and its workspace.
 struct TilePlan {
   int seq_begin, n_seqs, max_q;
-  int rw;                   // 32-row groups of a unit: 1, 2 or 4
-  int grid, whole, slot_rows;
+  int rw;                   // tile kernel: 32-row groups of a unit, 1, 2 or 4; 0: narrow kernel
+  int grid, ranges;         // workgroups; ranges the list is split into
+  int whole, slot_rows;
   size_t head_bytes, ml_bytes, acc_bytes;
 };
 

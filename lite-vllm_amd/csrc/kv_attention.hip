@@ -187,9 +187,10 @@ int device_cus() {
 }
 
 // How the sequences of a part are launched.  Everything here follows from the
-// sizes the caller names, never from what is in device memory.
+// sizes the caller names, never from what is in device memory.  `codes`: an
+// 8-bit cache whose strides the narrow kernel takes.
 TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num_kv_heads,
-                    int head_dim, int max_blocks, lv_dtype dtype) {
+                    int head_dim, int max_blocks, lv_dtype dtype, bool codes) {
   TilePlan p{};
   p.seq_begin = seq_begin;
   p.n_seqs = n_seqs;
@@ -201,14 +202,21 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_blocks * kBs + kt - 1) / kt);
   // contexts of a few tiles: splitting them costs more than it gives
   p.whole = tiles <= 4;
-  const int64_t resident = (int64_t)device_cus() * (dtype == LV_F32 ? 1 : 2);
+  const int64_t cus = device_cus();
   p.grid = (int)(p.whole ? std::min<int64_t>(units, 1 << 20)
-                         : std::min<int64_t>(units * tiles, resident));
+                         : std::min<int64_t>(units * tiles, cus * (dtype == LV_F32 ? 1 : 2)));
+  p.ranges = p.grid;
+  if (codes && dtype != LV_F32 && rows <= 8 && !p.whole) {
+    p.rw = 0;
+    const int64_t narrow = (int64_t)n_seqs * num_kv_heads * ((max_blocks + 1) / 2);
+    p.grid = (int)std::min<int64_t>((narrow + 3) / 4, cus * 2);
+    p.ranges = 4 * p.grid;
+  }
   p.slot_rows = (int)std::min<int64_t>(rows, r);
   if (!p.whole) {
-    p.head_bytes = align256((size_t)p.grid * 2 * 16);
-    p.ml_bytes = align256((size_t)2 * p.grid * p.slot_rows * 8);
-    p.acc_bytes = align256((size_t)2 * p.grid * p.slot_rows * head_dim * 4);
+    p.head_bytes = align256((size_t)p.ranges * 2 * 16);
+    p.ml_bytes = align256((size_t)2 * p.ranges * p.slot_rows * 8);
+    p.acc_bytes = align256((size_t)2 * p.ranges * p.slot_rows * head_dim * 4);
   }
   return p;
 }
@@ -217,15 +225,18 @@ size_t plan_bytes(const TilePlan& p) { return p.head_bytes + p.ml_bytes + p.acc_
 
 size_t workspace_size(int num_seqs, int num_decodes, int max_query_len, int num_heads,
                       int num_kv_heads, int head_dim, int max_blocks, lv_dtype dtype) {
+  // (of an 8-bit cache or not: the larger need)
   if (num_seqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || max_blocks < 0) return 0;
   size_t need = 0;
-  if (num_decodes > 0)
-    need = plan_bytes(plan_tiles(0, num_decodes, 1, num_heads, num_kv_heads, head_dim, max_blocks,
-                                 dtype));
-  if (num_seqs > num_decodes)
-    need = std::max(need, plan_bytes(plan_tiles(num_decodes, num_seqs - num_decodes,
-                                                max_query_len, num_heads, num_kv_heads, head_dim,
-                                                max_blocks, dtype)));
+  for (const bool codes : {false, true}) {
+    if (num_decodes > 0)
+      need = std::max(need, plan_bytes(plan_tiles(0, num_decodes, 1, num_heads, num_kv_heads,
+                                                  head_dim, max_blocks, dtype, codes)));
+    if (num_seqs > num_decodes)
+      need = std::max(need, plan_bytes(plan_tiles(num_decodes, num_seqs - num_decodes,
+                                                  max_query_len, num_heads, num_kv_heads,
+                                                  head_dim, max_blocks, dtype, codes)));
+  }
   return need;
 }
 
@@ -238,14 +249,15 @@ int launch_part(const Call& a, const TilePlan& p, char* ws) {
 int launch(const Call& a, int num_decodes, int max_query_len, void* ws) {
   const int h = a.r.num_heads, hkv = a.r.num_kv_heads, mb = a.b.max_blocks;
   if (a.code < 0 && a.dtype == LV_F32) return launch_rows(a);
-  if (num_decodes > 0)
-    if (const int rc = launch_part(a, plan_tiles(0, num_decodes, 1, h, hkv, a.d, mb, a.dtype),
-                                   (char*)ws);
-        rc != LV_OK)
-      return rc;
+  // (the narrow kernel's offsets within a block are 32 bits wide)
+  const bool codes = a.code >= 0 && a.c.tok <= (1 << 26);
+  if (num_decodes > 0) {
+    const TilePlan p = plan_tiles(0, num_decodes, 1, h, hkv, a.d, mb, a.dtype, codes);
+    if (const int rc = launch_part(a, p, (char*)ws); rc != LV_OK) return rc;
+  }
   if (num_decodes == a.b.num_seqs) return LV_OK;
   return launch_part(a, plan_tiles(num_decodes, a.b.num_seqs - num_decodes, max_query_len, h, hkv,
-                                   a.d, mb, a.dtype),
+                                   a.d, mb, a.dtype, codes),
                      (char*)ws);
 }
 

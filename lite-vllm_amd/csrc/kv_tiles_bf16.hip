@@ -1,5 +1,5 @@
-// The tile attention kernels for bf16 queries.
-#include "kv_tiles.h"
+// The attention kernels over paged caches for bf16 queries.
+#include "kv_launch.h"
 
 namespace lv {
 

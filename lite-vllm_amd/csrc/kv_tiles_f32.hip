@@ -1,5 +1,5 @@
-// The tile attention kernels for fp32 queries.
-#include "kv_tiles.h"
+// The attention kernels over paged caches for fp32 queries.
+#include "kv_launch.h"
 
 namespace lv {
 

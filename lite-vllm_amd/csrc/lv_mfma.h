@@ -100,6 +100,10 @@ __device__ __forceinline__ void load_lds16_stream(uint64_t base, uint32_t offset
                "s"(base)
                : "memory");
 }
+// 4 bytes per lane from any address, at byte address lds + 4 lane.
+__device__ __forceinline__ void load_lds4_async(const void* g, uint32_t lds) {
+  asm volatile(LV_SET_M0("%1") "global_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory");
+}
 #undef LV_SET_M0
 
 // Waits until at most N of the wavefront's vector-memory operations are
