@@ -84,8 +84,8 @@ struct Call {
 struct TilePlan {
   int seq_begin, n_seqs, max_q;
   int rw;                   // tile kernel: 32-row groups of a unit, 1, 2 or 4; 0: narrow kernel
-  int grid, ranges;         // workgroups; ranges the list is split into
-  int whole, slot_rows;
+  int grid;                 // workgroups, and ranges that the list is split into
+  int whole, slot_heads, slot_rows;
   size_t head_bytes, ml_bytes, acc_bytes;
 };
 

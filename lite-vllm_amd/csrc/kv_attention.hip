@@ -205,18 +205,20 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   const int64_t cus = device_cus();
   p.grid = (int)(p.whole ? std::min<int64_t>(units, 1 << 20)
                          : std::min<int64_t>(units * tiles, cus * (dtype == LV_F32 ? 1 : 2)));
-  p.ranges = p.grid;
+  p.slot_heads = 1;
+  p.slot_rows = (int)std::min<int64_t>(rows, r);
   if (codes && dtype != LV_F32 && rows <= 8 && !p.whole) {
     p.rw = 0;
-    const int64_t narrow = (int64_t)n_seqs * num_kv_heads * ((max_blocks + 1) / 2);
-    p.grid = (int)std::min<int64_t>((narrow + 3) / 4, cus * 2);
-    p.ranges = 4 * p.grid;
+    p.slot_heads = std::min(num_kv_heads, 8);
+    while (num_kv_heads % p.slot_heads != 0) --p.slot_heads;
+    const int64_t list = (int64_t)n_seqs * (num_kv_heads / p.slot_heads) * ((max_blocks + 1) / 2);
+    p.grid = (int)std::min<int64_t>(list, cus * (8 / p.slot_heads));
   }
-  p.slot_rows = (int)std::min<int64_t>(rows, r);
   if (!p.whole) {
-    p.head_bytes = align256((size_t)p.ranges * 2 * 16);
-    p.ml_bytes = align256((size_t)2 * p.ranges * p.slot_rows * 8);
-    p.acc_bytes = align256((size_t)2 * p.ranges * p.slot_rows * head_dim * 4);
+    const size_t slots = (size_t)2 * p.grid * p.slot_heads * p.slot_rows;
+    p.head_bytes = align256((size_t)p.grid * 2 * 16);
+    p.ml_bytes = align256(slots * 8);
+    p.acc_bytes = align256(slots * head_dim * 4);
   }
   return p;
 }

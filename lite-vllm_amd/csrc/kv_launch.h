@@ -11,6 +11,7 @@ inline TileArgs tile_args(const Call& a, const TilePlan& p, char* ws) {
   t.b = a.b; t.c = a.c; t.r = a.r;
   t.seq_begin = p.seq_begin; t.n_seqs = p.n_seqs; t.max_q = p.max_q;
   t.whole = p.whole;
+  t.slot_heads = p.slot_heads;
   t.slot_rows = p.slot_rows;
   t.head = reinterpret_cast<int4*>(ws);
   t.ml = reinterpret_cast<float*>(ws + p.head_bytes);
@@ -21,9 +22,10 @@ inline TileArgs tile_args(const Call& a, const TilePlan& p, char* ws) {
 template <typename T, int D>
 int launch_join(const Call& a, const TilePlan& p, const TileArgs& t) {
   constexpr int TEAMS = 256 / (D / 4);
-  int rows_per = 1;
-  while (rows_per < TEAMS && rows_per * 2 < p.slot_rows) rows_per *= 2;
-  attn_join_kernel<T, D><<<dim3((unsigned)p.ranges - 1, (unsigned)((p.slot_rows + rows_per - 1) / rows_per)),
+  // few rows may have many pieces: the teams share them
+  const int rows = p.slot_heads * p.slot_rows;
+  const int rows_per = p.slot_rows <= 8 ? 1 : TEAMS;
+  attn_join_kernel<T, D><<<dim3((unsigned)p.grid - 1, (unsigned)((rows + rows_per - 1) / rows_per)),
                            256, 0, a.stream>>>(t, rows_per);
   return check_launch("attn_join_kernel");
 }
@@ -34,7 +36,7 @@ int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
   const TileArgs t = tile_args(a, p, ws);
   const size_t lds = (size_t)F::KT * D * 4 + F::KT * 8 + 128 * 8 + (size_t)(p.n_seqs + 1) * 4;
   attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, kTileThreads, lds, a.stream>>>(t);
-  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.whole || p.ranges < 2)
+  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.whole || p.grid < 2)
     return rc;
   return launch_join<T, D>(a, p, t);
 }
@@ -42,8 +44,9 @@ int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
 template <typename T, typename C, int D, bool TREE>
 int launch_narrow_kernel(const Call& a, const TilePlan& p, char* ws) {
   const TileArgs t = tile_args(a, p, ws);
-  const size_t lds = (size_t)4 * 2 * NarrowStage<D>::BYTES + (size_t)(p.n_seqs + 1) * 4;
-  attn_narrow_kernel<T, C, D, TREE><<<(unsigned)p.grid, kTileThreads, lds, a.stream>>>(t);
+  const size_t lds = (size_t)p.slot_heads * 2 * NarrowStage<D>::BYTES + (size_t)(p.n_seqs + 1) * 4;
+  attn_narrow_kernel<T, C, D, TREE>
+      <<<(unsigned)p.grid, (unsigned)(64 * p.slot_heads), lds, a.stream>>>(t);
   if (const int rc = check_launch("attn_narrow_kernel"); rc != LV_OK) return rc;
   return launch_join<T, D>(a, p, t);
 }

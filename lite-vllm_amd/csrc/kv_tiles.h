@@ -48,10 +48,10 @@ struct TileArgs {
   Batch b; KvView c; Rows r;
   int seq_begin, n_seqs, max_q;
   int whole;                // ranges of whole units: nothing to join
-  int slot_rows;            // rows of a workspace slot
-  int4* head;               // [grid][2]: the unit that crosses a range's start
-  float* ml;                // [2 grid][slot_rows][2]
-  float* acc;               // [2 grid][slot_rows][D]
+  int slot_heads, slot_rows;   // kv heads of a workspace slot, rows of each
+  int4* head;               // [ranges][2]: the unit that crosses a range's start
+  float* ml;                // [2 ranges][slot_heads][slot_rows][2]
+  float* acc;               // [2 ranges][slot_heads][slot_rows][D]
 };
 
 struct Unit { int seq, q0, n, rows, committed, kend, kvh, row0, ntiles; };
@@ -224,6 +224,15 @@ __device__ __forceinline__ uint32_t take_part(float& a, float& b, bool last) {
   }
 }
 
+// Waits here for the loads of these registers.  Left alone, the compiler waits
+// at their first use, which lies in a loop, and so on every pass for whatever
+// loads are then in flight.
+template <int N>
+__device__ __forceinline__ void settle(uint4 (&q)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(q[i].x), "+v"(q[i].y), "+v"(q[i].z), "+v"(q[i].w));
+}
+
 __device__ __forceinline__ void team_barrier() {
   wait_lds();                      // (loads into registers stay in flight)
   __builtin_amdgcn_s_barrier();
@@ -394,11 +403,16 @@ void attn_tile_kernel(TileArgs a) {
     qhead = u.kvh * G + use % G;
     lim = TREE ? u.kend - 1 : min(u.committed + use / G, u.kend - 1);
     const T* qp = (const T*)a.r.q + (int64_t)qrow * a.r.q_stride + (int64_t)qhead * D + 8 * h;
+    if constexpr (P::QP == 1) {
+      uint4 raw[QSTEPS];
 #pragma unroll
-    for (int s = 0; s < QSTEPS; ++s) {
-      if constexpr (P::QP == 1) {
-        qf[0][s] = __builtin_bit_cast(qv8, load16(qp + 16 * s));
-      } else {
+      for (int s = 0; s < QSTEPS; ++s) raw[s] = load16(qp + 16 * s);
+      settle(raw);
+#pragma unroll
+      for (int s = 0; s < QSTEPS; ++s) qf[0][s] = __builtin_bit_cast(qv8, raw[s]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < QSTEPS; ++s) {
         float x[8];
         elem<float>::unpack(load16(qp + 16 * s), x);
         elem<float>::unpack(load16(qp + 16 * s + 4), x + 4);
@@ -717,6 +731,7 @@ void attn_tile_kernel(TileArgs a) {
     const bool more = inside || p + 1 < r1;
     Unit N = U;
     int nt = t + 1;
+    if (fresh) start(U);
     if (more) {
       if (!inside) {
         N = next_unit<TREE, RW>(a, U, G);
@@ -724,7 +739,6 @@ void attn_tile_kernel(TileArgs a) {
       }
       load_tile(N, nt, !inside);
     }
-    if (fresh) start(U);
     if constexpr (RW > 1) team_barrier();
     else wait_lds();
     compute(U, t);
@@ -744,10 +758,12 @@ void attn_tile_kernel(TileArgs a) {
 // the unit that crosses the start of range w and begins in range w - 1, its
 // rows rows_per y ...  Its pieces lie in slots 2 (w - 1) + 1, 2 w, 2 (w + 1),
 // ...  D / 4 lanes per row, `rows_per` rows at a time, the rest of the
-// workgroup the row's other pieces.
+// workgroup the row's other pieces; four pieces' loads are in flight at once
+// (two sequences of 131000 tokens over 2048 ranges, 128 pieces a row: 18.5 ->
+// JOINUS us).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(TileArgs a, int rows_per) {
-  constexpr int LPR = D / 4, TEAMS = 256 / LPR;
+  constexpr int LPR = D / 4, TEAMS = 256 / LPR, U = 4;
   __shared__ float2 s_ml[TEAMS];
   __shared__ float4 s_o[TEAMS][LPR];
   const int w = blockIdx.x + 1;
@@ -756,19 +772,32 @@ __global__ __launch_bounds__(256) void attn_join_kernel(TileArgs a, int rows_per
   const int nrows = a.head[2 * w + 1].x;
   const int team = threadIdx.x / LPR, d = 4 * (threadIdx.x % LPR);
   const int parts = TEAMS / rows_per;          // pieces taken side by side
-  const int row = (int)blockIdx.y * rows_per + team / parts;
-  const bool on = row < nrows;
+  const int slot_rows = a.slot_heads * a.slot_rows;
+  const int row = (int)blockIdx.y * rows_per + team / parts;   // of the slot
+  const int head = row / a.slot_rows, own = row - head * a.slot_rows;
+  const bool on = head < a.slot_heads && own < nrows;
   float m = kNegBig, l = 0.0f, o[4] = {};
+  auto fold = [&](const float2& ml, const float4& v, float weight) {
+    const float mn = fmaxf(m, ml.x), f0 = fast_exp2(m - mn), f1 = weight * fast_exp2(ml.x - mn);
+    m = mn;
+    l = l * f0 + ml.y * fast_exp2(ml.x - mn);
+    o[0] = o[0] * f0 + v.x * f1; o[1] = o[1] * f0 + v.y * f1;
+    o[2] = o[2] * f0 + v.z * f1; o[3] = o[3] * f0 + v.w * f1;
+  };
   if (on) {
-    for (int i = team % parts; i < hd.x; i += parts) {
-      const int64_t slot = i == 0 ? 2 * (w - 1) + 1 : 2 * (w - 1 + i);
-      const float2 ml = *reinterpret_cast<const float2*>(a.ml + (slot * a.slot_rows + row) * 2);
-      const float4 v = *reinterpret_cast<const float4*>(a.acc + (slot * a.slot_rows + row) * D + d);
-      const float mn = fmaxf(m, ml.x), f0 = fast_exp2(m - mn), f1 = ml.y * fast_exp2(ml.x - mn);
-      m = mn;
-      l = l * f0 + f1;
-      o[0] = o[0] * f0 + v.x * f1; o[1] = o[1] * f0 + v.y * f1;
-      o[2] = o[2] * f0 + v.z * f1; o[3] = o[3] * f0 + v.w * f1;
+    for (int i = team % parts; i < hd.x; i += U * parts) {
+      float2 ml[U];
+      float4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int e = min(i + u * parts, hd.x - 1);
+        const int64_t slot = e == 0 ? 2 * (w - 1) + 1 : 2 * (w - 1 + e);
+        ml[u] = *reinterpret_cast<const float2*>(a.ml + (slot * slot_rows + row) * 2);
+        v[u] = *reinterpret_cast<const float4*>(a.acc + (slot * slot_rows + row) * D + d);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * parts < hd.x) fold(ml[u], v[u], ml[u].y);
     }
   }
   if (parts > 1) {
@@ -776,22 +805,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(TileArgs a, int rows_per
     s_o[team][d / 4] = make_float4(o[0], o[1], o[2], o[3]);
     __syncthreads();
     if (team % parts != 0 || !on) return;
-    for (int k = 1; k < parts; ++k) {
-      const float2 ml = s_ml[team + k];
-      const float4 v = s_o[team + k][d / 4];
-      const float mn = fmaxf(m, ml.x), f0 = fast_exp2(m - mn), f1 = fast_exp2(ml.x - mn);
-      m = mn;
-      l = l * f0 + ml.y * f1;
-      o[0] = o[0] * f0 + v.x * f1; o[1] = o[1] * f0 + v.y * f1;
-      o[2] = o[2] * f0 + v.z * f1; o[3] = o[3] * f0 + v.w * f1;
-    }
+    for (int k = 1; k < parts; ++k) fold(s_ml[team + k], s_o[team + k][d / 4], 1.0f);
   }
   if (!on) return;
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   const int g = a.r.num_heads / a.r.num_kv_heads;
-  const int idx = hd.w + row;
+  const int idx = hd.w + own;
   T* op = (T*)a.r.out + (int64_t)(hd.y + idx / g) * a.r.out_stride +
-          (int64_t)(hd.z * g + idx % g) * D + d;
+          (int64_t)((hd.z + head) * g + idx % g) * D + d;
 #pragma unroll
   for (int i = 0; i < 4; ++i) elem<T>::store(op + i, o[i] * inv);
 }
