@@ -34,7 +34,7 @@ template <typename T, typename C, int D, int RW, bool TREE>
 int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
   using F = TileCfg<RW>;
   const TileArgs t = tile_args(a, p, ws);
-  const size_t lds = (size_t)F::KT * D * 4 + F::KT * 8 + 128 * 8 + (size_t)(p.n_seqs + 1) * 4;
+  const size_t lds = F::lds(D) + (size_t)(p.n_seqs + 1) * 4;
   attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, kTileThreads, lds, a.stream>>>(t);
   if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.whole || p.grid < 2)
     return rc;

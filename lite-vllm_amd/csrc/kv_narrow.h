@@ -7,7 +7,7 @@
 // the kv heads (up to 8): they walk the same tiles side by side, so that a
 // block's rows of all heads, one run of memory, are read together (a wavefront
 // with a range of its own over one head's tiles reads runs of 2 KiB and half
-// lines of scales: 110 us for 256 sequences of 16-2048 tokens against DECUS).
+// lines of scales: 110 us for 256 sequences of 16-2048 tokens against 96).
 // A barrier every few tiles, with no wait for loads, keeps them together.
 //   * Codes and scales go from HBM to LDS directly (global_load_lds), two
 //     stages of one tile, waits by vmcnt; tile i + 1 is in flight while tile i

@@ -29,12 +29,19 @@ namespace lv {
 //   * S^T = K Q^T, v_mfma_f32_32x32x16: a lane ends with one query row (its
 //     column) against 16 of each 32 keys;
 //   * x = S^T * (scale of the key's row * scale), masked by position or tree;
-//     running maximum (raised only when passed by 2^8), weights and their sum
-//     in fp32;
-//   * O^T += V^T P^T with P = weight * scale of the value's row.  P is split
-//     into PP bf16 (fp16 cache: fp16) parts, each a product of its own: two
-//     hold 16 bits (2^-17 of a weight), three all of fp32.  One part (2^-9)
-//     would add an error as large as the output's own rounding.
+//     maximum (raised rarely), weights and their sum in fp32;
+//   * O^T += V^T P^T with P = weight * scale of the value's row.
+// P would lose 2^-9 of each weight as bf16, an error as large as that of a
+// bf16 output.  16-bit queries over codes: P is one fp16 value (2^-12).  With
+// y = x + log2(scale of the value's row), P = exp2(y - reference) takes no
+// multiplication, the weights' sum is sum P / scale, and the reference follows
+// the largest y, so that the largest P of a row is between 2^10 and 2^15
+// whatever the scales are.  (Against two bf16 parts, 48 products a tile instead
+// of 32 and 12 vector instructions a score instead of 9: 462 -> 390 us
+// for two chunks of 700-1024 tokens at 15000-19000, 8 query heads a kv head.)
+// Scales outside [2^-60, 2^20] of the unit's first ones, and ones that are not
+// finite, make the piece careful (below).  fp32 queries: three bf16 parts, all
+// the bits.  A bf16 cache: two (2^-17), an fp16 cache: one fp16 value.
 // fp32 queries are three bf16 parts (all their bits), others are taken as
 // they are.
 //
@@ -54,13 +61,20 @@ struct TileArgs {
   float* acc;               // [2 ranges][slot_heads][slot_rows][D]
 };
 
-struct Unit { int seq, q0, n, rows, committed, kend, kvh, row0, ntiles; };
+struct Unit {
+  int seq, q0, n, rows, committed, kend, kvh, row0, ntiles;
+  int unit2;     // the V scales' unit is 2^unit2 (16-bit queries over codes)
+};
 
 template <int RW> struct TileCfg {
   static constexpr int R = 32 * RW, KW = 4 / RW;
   static constexpr int KT = RW == 4 ? 64 : 128;   // keys per tile
   static constexpr int BPW = KT / 64;             // 16-token blocks a wavefront stages
   static constexpr int KPW = KT / KW;             // keys a wavefront computes
+  static constexpr int NST = RW == 4 ? 2 : 1;     // LDS stages
+  static constexpr size_t lds(int d) {            // without the list's offsets
+    return (size_t)NST * (KT * d * 4 + KT * 12) + 128 * 8;
+  }
 };
 
 // Keys that row tile [row0, row0 + R) of a sequence needs.
@@ -233,6 +247,8 @@ __device__ __forceinline__ void settle(uint4 (&q)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(q[i].x), "+v"(q[i].y), "+v"(q[i].z), "+v"(q[i].w));
 }
 
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
 __device__ __forceinline__ void team_barrier() {
   wait_lds();                      // (loads into registers stay in flight)
   __builtin_amdgcn_s_barrier();
@@ -242,13 +258,17 @@ __device__ __forceinline__ void team_barrier() {
 template <typename T, typename C> struct Operands {
   static constexpr bool kCodes = cached<C>::kCodes;
   using K = typename std::conditional<std::is_same<T, f16>::value, f16, bf16>::type;
-  using V = typename std::conditional<kCodes, bf16, K>::type;
-  static constexpr int QP = std::is_same<T, float>::value ? 3 : 1;
-  static constexpr int PP = std::is_same<T, float>::value ? 3 : 2;
-  // fp16 weights: the reference lies 2^7 under the maximum that set it, so that
-  // a row's largest weight is between 2^7 and 2^15 and the fixed step of the
-  // smallest fp16 values weighs little against it
-  static constexpr float kLift = std::is_same<V, f16>::value ? 7.0f : 0.0f;
+  static constexpr bool kF32 = std::is_same<T, float>::value;
+  static constexpr bool kLog = kCodes && !kF32;   // P = exp2(x + log2 of V's scale)
+  using V = typename std::conditional<kCodes, typename std::conditional<kF32, bf16, f16>::type,
+                                      K>::type;
+  static constexpr int QP = kF32 ? 3 : 1;
+  static constexpr int PP = kF32 ? 3 : std::is_same<V, f16>::value ? 1 : 2;
+  // A row's reference is set kLift (in log2 units) under the score that sets it
+  // and again when a score passes it by kTop: fp16 weights then lie high enough
+  // that the fixed step of the smallest ones, 2^-24, weighs nothing.
+  static constexpr float kLift = std::is_same<V, f16>::value ? 10.0f : 0.0f;
+  static constexpr float kTop = std::is_same<V, f16>::value ? 15.0f : 8.0f;
 };
 
 // Workgroups per CU: the three parts of fp32 queries need the registers of two.
@@ -274,11 +294,11 @@ void attn_tile_kernel(TileArgs a) {
   // K and V tile, then the scales of its keys; the merge of a piece's parts
   // reuses the tiles (4 wavefronts x 32 rows x D floats at most)
   extern __shared__ __align__(16) unsigned char s_dyn[];
-  uint16_t* const Ks = reinterpret_cast<uint16_t*>(s_dyn);
-  uint16_t* const Vs = Ks + KT * D;
-  float* const s_ks = reinterpret_cast<float*>(Vs + KT * D);
-  float* const s_vs = s_ks + KT;
-  float2* const s_ml = reinterpret_cast<float2*>(s_vs + KT);   // [4][32]
+  constexpr int NST = F::NST, TILE = KT * D;       // (elements of K or V)
+  uint16_t* const s_kv = reinterpret_cast<uint16_t*>(s_dyn);       // [NST][K, V][TILE]
+  // [NST][KT] each: K's scales; V's scales, or their logarithms and inverses
+  float* const s_sc = reinterpret_cast<float*>(s_kv + NST * 2 * TILE);
+  float2* const s_ml = reinterpret_cast<float2*>(s_sc + NST * 3 * KT);   // [4][32]
   int* const s_off = reinterpret_cast<int*>(s_ml + 128);
   __shared__ int s_part[4];
 
@@ -330,8 +350,22 @@ void attn_tile_kernel(TileArgs a) {
     }
     id_first = first;
   };
-  auto load_tile = [&](const Unit& u, int tile, bool fresh) {
+  auto load_tile = [&](Unit& u, int tile, bool fresh) {
     if (fresh || tile - id_first >= 64) load_ids(u, tile);
+    if constexpr (P::kLog) {
+      if (fresh) {       // the unit of the V scales: the largest of the first 64
+        float v = 0.0f;
+        const int key = tile * KT + lane;
+        if (key < u.kend) {
+          const int64_t phys =
+              physical_block(a.b, a.c.num_blocks, a.seq_begin + u.seq, key / kBs);
+          v = a.c.scale[1][phys * a.c.sblk + (key % kBs) * a.c.stok + u.kvh * a.c.shead];
+        }
+        v = group_max<64>(v > 0.0f && v < __builtin_inff() ? v : 0.0f);
+        const int e = (int)(__builtin_amdgcn_readfirstlane(__float_as_uint(v)) >> 23) - 127;
+        u.unit2 = v > 0.0f ? min(max(e, -100), 100) : 0;
+      }
+    }
     int phys[BPW];     // (read by all lanes: a readlane under a branch sees stale copies)
 #pragma unroll
     for (int j = 0; j < BPW; ++j) phys[j] = __builtin_amdgcn_readlane(ids[j], tile - id_first);
@@ -356,7 +390,9 @@ void attn_tile_kernel(TileArgs a) {
       sraw = base[block * a.c.sblk + (key & 15) * a.c.stok + u.kvh * a.c.shead];
     }
   };
-  auto write_tile = [&](const Unit& u, int tile) {
+  auto write_tile = [&](const Unit& u, int tile, int st) {
+    uint16_t* const Ks = s_kv + st * 2 * TILE;
+    uint16_t* const Vs = Ks + TILE;
     const int key0 = tile * KT + wave * 16 * BPW;
     const bool tail = key0 + 16 * BPW > u.kend;
 #pragma unroll
@@ -382,8 +418,20 @@ void attn_tile_kernel(TileArgs a) {
     if constexpr (kCodes) {
       const int key = lane % (16 * BPW), kv = lane / (16 * BPW);
       const int row = 16 * wave * BPW + key;
-      if (kv == 0) s_ks[row] = sraw * a.r.scale_log2;
-      if (kv == 1) s_vs[row] = tile * KT + row < u.kend ? sraw : 0.0f;
+      float* const sc = s_sc + st * 3 * KT;
+      const bool in = tile * KT + row < u.kend;
+      if (kv == 0) sc[row] = sraw * a.r.scale_log2;
+      if (kv == 1) {
+        if constexpr (P::kLog) {
+          const float v = sraw * pow2(-u.unit2);
+          const bool ok = v >= 0x1p-60f && v <= 0x1p20f;
+          sc[KT + row] = !in ? 0.0f : ok ? __builtin_amdgcn_logf(v) : v == 0.0f ? -60.0f : 0.0f;
+          sc[2 * KT + row] = !in ? 0.0f : ok ? __builtin_amdgcn_rcpf(v)
+                                       : v == 0.0f ? 0x1p60f : __builtin_nanf("");
+        } else {
+          sc[KT + row] = in ? sraw : 0.0f;
+        }
+      }
     }
   };
 
@@ -463,21 +511,34 @@ void attn_tile_kernel(TileArgs a) {
     return (uint32_t)v;
   };
 
-  auto compute = [&](const Unit& u, int tile) {
+  auto compute = [&](const Unit& u, int tile, int st) {
     const int k0 = tile * KT + kg * KPW;           // this wavefront's first key
-    const uint16_t* kt = Ks + kg * KPW * D;
-    const uint16_t* vt = Vs + kg * KPW * D;
+    const uint16_t* kt = s_kv + st * 2 * TILE + kg * KPW * D;
+    const uint16_t* vt = kt + TILE;
+    const float* const s_ks = s_sc + st * 3 * KT + kg * KPW;
+    const float* const s_vs = s_ks + KT;
+    // Four K operands in flight: read j + 4 goes out when product j has taken
+    // its buffer (left to itself, the compiler waits out each read in turn).
     f32x16_t sv[KB];
+    {
+      constexpr int NJ = KB * QSTEPS;
+      auto kread = [&](int j) __attribute__((always_inline)) {
+        return *reinterpret_cast<const uint4*>(kt + 32 * (j / QSTEPS) * D + kx[j % QSTEPS]);
+      };
+      uint4 ka[4];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
+      for (int j = 0; j < 4; ++j) ka[j] = kread(j);
 #pragma unroll
-      for (int s = 0; s < QSTEPS; ++s) {
-        const qv8 kf = __builtin_bit_cast(
-            qv8, *reinterpret_cast<const uint4*>(kt + 32 * kb * D + kx[s]));
+      for (int j = 0; j < NJ; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int kb = j / QSTEPS, s = j % QSTEPS;
 #pragma unroll
         for (int p = P::QP - 1; p >= 0; --p)       // the small parts first
-          sv[kb] = KM::run(kf, qf[p][s], s || p + 1 < P::QP ? sv[kb] : f32x16_t{});
+          sv[kb] = KM::run(__builtin_bit_cast(qv8, ka[j & 3]), qf[p][s],
+                           s || p + 1 < P::QP ? sv[kb] : f32x16_t{});
+        if (j + 4 < NJ) ka[j & 3] = kread(j + 4);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     // x in log2 units; the first key that some row may not see
     float mx = kNegBig;
@@ -486,9 +547,14 @@ void attn_tile_kernel(TileArgs a) {
       if constexpr (kCodes) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          const float4 ks = *reinterpret_cast<const float4*>(s_ks + kg * KPW + 32 * kb + 8 * q4 + 4 * h);
-          sv[kb][4 * q4] *= ks.x; sv[kb][4 * q4 + 1] *= ks.y;
-          sv[kb][4 * q4 + 2] *= ks.z; sv[kb][4 * q4 + 3] *= ks.w;
+          const float4 ks = *reinterpret_cast<const float4*>(s_ks + 32 * kb + 8 * q4 + 4 * h);
+          float4 add = make_float4(0, 0, 0, 0);
+          if constexpr (P::kLog)
+            add = *reinterpret_cast<const float4*>(s_vs + 32 * kb + 8 * q4 + 4 * h);
+          sv[kb][4 * q4] = fmaf(sv[kb][4 * q4], ks.x, add.x);
+          sv[kb][4 * q4 + 1] = fmaf(sv[kb][4 * q4 + 1], ks.y, add.y);
+          sv[kb][4 * q4 + 2] = fmaf(sv[kb][4 * q4 + 2], ks.z, add.z);
+          sv[kb][4 * q4 + 3] = fmaf(sv[kb][4 * q4 + 3], ks.w, add.w);
         }
       } else {
 #pragma unroll
@@ -517,7 +583,7 @@ void attn_tile_kernel(TileArgs a) {
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sv[kb][i]);
     mx = xor32_max(mx);
     float alpha = 1.0f;
-    if (mx > m_run + P::kLift + 8.0f) {
+    if (mx > m_run + P::kTop) {
       alpha = fast_exp2(m_run - (mx - P::kLift));
       m_run = mx - P::kLift;
     }
@@ -531,16 +597,26 @@ void attn_tile_kernel(TileArgs a) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        sv[kb][i] = fast_exp2(sv[kb][i] - m_run);
-        l_run += sv[kb][i];
-      }
-      if constexpr (kCodes) {
+      for (int i = 0; i < 16; ++i) sv[kb][i] = fast_exp2(sv[kb][i] - m_run);
+      if constexpr (P::kLog) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          const float4 vs = *reinterpret_cast<const float4*>(s_vs + kg * KPW + 32 * kb + 8 * q4 + 4 * h);
-          sv[kb][4 * q4] *= vs.x; sv[kb][4 * q4 + 1] *= vs.y;
-          sv[kb][4 * q4 + 2] *= vs.z; sv[kb][4 * q4 + 3] *= vs.w;
+          const float4 rv = *reinterpret_cast<const float4*>(s_vs + KT + 32 * kb + 8 * q4 + 4 * h);
+          l_run = fmaf(sv[kb][4 * q4], rv.x, l_run);
+          l_run = fmaf(sv[kb][4 * q4 + 1], rv.y, l_run);
+          l_run = fmaf(sv[kb][4 * q4 + 2], rv.z, l_run);
+          l_run = fmaf(sv[kb][4 * q4 + 3], rv.w, l_run);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) l_run += sv[kb][i];
+        if constexpr (kCodes) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const float4 vs = *reinterpret_cast<const float4*>(s_vs + 32 * kb + 8 * q4 + 4 * h);
+            sv[kb][4 * q4] *= vs.x; sv[kb][4 * q4 + 1] *= vs.y;
+            sv[kb][4 * q4 + 2] *= vs.z; sv[kb][4 * q4 + 3] *= vs.w;
+          }
         }
       }
       uint32_t pw[P::PP][8];
@@ -652,18 +728,21 @@ void attn_tile_kernel(TileArgs a) {
     }
   };
   auto finish = [&](const Unit& u, int t0, int t1) {
-    float all = 0.0f;
+    float all = l_run, unit = P::kLog ? pow2(u.unit2) : 1.0f;
 #pragma unroll
     for (int b = 0; b < DBLK; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) all += o[b][i];
-    if (__ballot(!(fabsf(all) < __builtin_inff()))) careful(u, t0, t1);
+    if (__ballot(!(fabsf(all) < __builtin_inff()))) {
+      careful(u, t0, t1);
+      unit = 1.0f;
+    }
     const bool whole = t0 == 0 && t1 == u.ntiles;
     const int slot = whole ? -1 : 2 * w + (t0 == 0 ? 1 : 0);
     const int idx = 32 * rg + lr;                  // the row's place in the unit
     l_run = xor32_sum(l_run);
     if constexpr (KW == 1) {
-      const float inv = l_run != 0.0f ? 1.0f / l_run : 0.0f;
+      const float inv = l_run != 0.0f ? unit / l_run : 0.0f;
       if (!live) return;
       if (!whole && h == 0)
         *reinterpret_cast<float2*>(a.ml + ((int64_t)slot * a.slot_rows + idx) * 2) =
@@ -683,7 +762,8 @@ void attn_tile_kernel(TileArgs a) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
           xo[(wave * (DBLK * 4) + 4 * b + q4) * 64 + lane] =
-              make_float4(o[b][4 * q4], o[b][4 * q4 + 1], o[b][4 * q4 + 2], o[b][4 * q4 + 3]);
+              make_float4(o[b][4 * q4] * unit, o[b][4 * q4 + 1] * unit, o[b][4 * q4 + 2] * unit,
+                          o[b][4 * q4 + 3] * unit);
       if (h == 0) s_ml[wave * 32 + lr] = make_float2(m_run, l_run);
       team_barrier();
       float2 ml[KW];
@@ -721,36 +801,79 @@ void attn_tile_kernel(TileArgs a) {
   };
 
   // -- the range ---------------------------------------------------------------
-  load_tile(U, t, true);
+  // The tile after (u, tile) at place p of the list: true if there is one;
+  // `inside`: it belongs to the same unit.
+  auto advance = [&](Unit& u, int& tile, int& p, bool& inside) {
+    inside = tile + 1 < u.ntiles && (a.whole || p + 1 < r1);
+    if (inside) {
+      ++tile;
+      p += a.whole ? 0 : 1;
+      return true;
+    }
+    if (p + 1 >= r1) return false;
+    ++p;
+    u = next_unit<TREE, RW>(a, u, G);
+    tile = 0;
+    return true;
+  };
   int first = t, p = r0;
   bool fresh = true;
-  while (true) {
-    if constexpr (RW > 1) team_barrier();          // the last tile has been read
-    write_tile(U, t);
-    const bool inside = t + 1 < U.ntiles && (a.whole || p + 1 < r1);
-    const bool more = inside || p + 1 < r1;
+  load_tile(U, t, true);
+  if constexpr (NST == 2) {
+    // one tile computed, the next in registers on its way to the other stage,
+    // the one after that being loaded: one barrier per tile
     Unit N = U;
-    int nt = t + 1;
-    if (fresh) start(U);
-    if (more) {
-      if (!inside) {
-        N = next_unit<TREE, RW>(a, U, G);
-        nt = 0;
+    int nt = t, st = 0;
+    bool inside = false;
+    write_tile(U, t, 0);
+    bool more = advance(N, nt, p, inside);
+    if (more) load_tile(N, nt, !inside);
+    team_barrier();
+    while (true) {
+      Unit M = N;
+      int mt = nt;
+      bool then = false, minside = false;
+      if (fresh) start(U);
+      if (more) {
+        write_tile(N, nt, st ^ 1);
+        then = advance(M, mt, p, minside);
+        if (then) load_tile(M, mt, !minside);
       }
-      load_tile(N, nt, !inside);
+      compute(U, t, st);
+      fresh = !(more && inside);
+      if (fresh) {
+        finish(U, first, t + 1);
+        first = 0;
+      }
+      if (!more) break;
+      team_barrier();
+      U = N; t = nt;
+      N = M; nt = mt;
+      more = then; inside = minside;
+      st ^= 1;
     }
-    if constexpr (RW > 1) team_barrier();
-    else wait_lds();
-    compute(U, t);
-    fresh = !inside;
-    if (!inside) {
-      finish(U, first, t + 1);
-      first = 0;
+  } else {
+    while (true) {
+      if constexpr (RW > 1) team_barrier();        // the last tile has been read
+      write_tile(U, t, 0);
+      if (fresh) start(U);
+      Unit N = U;
+      int nt = t;
+      bool inside = false;
+      const bool more = advance(N, nt, p, inside);
+      if (more) load_tile(N, nt, !inside);
+      if constexpr (RW > 1) team_barrier();
+      else wait_lds();
+      compute(U, t, 0);
+      fresh = !(more && inside);
+      if (fresh) {
+        finish(U, first, t + 1);
+        first = 0;
+      }
+      if (!more) break;
+      U = N;
+      t = nt;
     }
-    if (!more) break;
-    if (!a.whole || !inside) ++p;
-    U = N;
-    t = nt;
   }
 }
 
@@ -760,7 +883,7 @@ void attn_tile_kernel(TileArgs a) {
 // ...  D / 4 lanes per row, `rows_per` rows at a time, the rest of the
 // workgroup the row's other pieces; four pieces' loads are in flight at once
 // (two sequences of 131000 tokens over 2048 ranges, 128 pieces a row: 18.5 ->
-// JOINUS us).
+// 9.6 us).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(TileArgs a, int rows_per) {
   constexpr int LPR = D / 4, TEAMS = 256 / LPR, U = 4;

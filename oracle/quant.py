@@ -62,15 +62,17 @@ def mask_words(sees: np.ndarray, words: int) -> np.ndarray:
 def attention(query, keys, values, sees, scale):
     """One sequence: query [n, H, D], keys / values [c, Hkv, D] float64, sees
     bool [n, c].  Returns (out, spread, reach): out [n, H, D]; spread, the
-    weighted sum of |v|, which a relative error of the weights multiplies; and
+    weighted sum of |v|, which a relative error of the weights multiplies;
     reach [n, H], the largest scale * sum |q| |k|, whose roundings are the
-    error of a score."""
+    error of a score; floor [n, H], the number of seen keys times the largest
+    |v| among them, which a fixed step of the weights multiplies."""
     q = query.detach().cpu().double()
     n, H, D = q.shape
     hkv = keys.shape[1]
     g = H // hkv
     out, spread = torch.zeros_like(q), torch.zeros_like(q)
     reach = torch.zeros(n, H, dtype=torch.float64)
+    floor = torch.zeros(n, H, dtype=torch.float64)
     seen = torch.as_tensor(sees)
     # (a key that nobody sees may hold anything)
     used = seen.any(0)
@@ -87,23 +89,32 @@ def attention(query, keys, values, sees, scale):
                 m = seen[j]
                 out[j, h] = w[j, m] @ v[m, h // g]
                 spread[j, h] = w[j, m] @ v[m, h // g].abs()
+                floor[j, h] = m.sum() * v[m, h // g].abs().max()
                 reach[j, h] = (abs(scale) * (q[j, h].abs() @ k[m, h // g].abs().T)).max()
-    return out, spread, reach
+    return out, spread, reach, floor
 
 
-def tolerance(out, spread, reach, dtype: torch.dtype):
+def tolerance(out, spread, reach, floor, dtype: torch.dtype):
     """How far a result of `dtype` may be off.
 
     Its own rounding: half a step of the result.  A score of D products summed
     in fp32 is off by at most (D + 4) 2^-24 of its reach (products, sums, and
     the scale's roundings), the weight by that relative amount, twice over
     through the sum of the weights; exp2 and the sums of weights and products
-    add at most 2^-20 for the lengths tested.  For 16-bit types the weights
-    may be rounded to 11 bits (2^-12 of each, again in numerator and, as the
-    sum takes them unrounded, not in the denominator)."""
+    add at most 2^-20 for the lengths tested.  For 16-bit types each weight may
+    be rounded to fp16 in the numerator (the sum takes it unrounded): half a
+    step of a value of 11 significant bits is 2^-11 of it where it is largest,
+    just above a power of two (1 + 2^-11 lies between 1 and 1 + 2^-10).
+    The smallest step of fp16 is 2^-24 whatever the value: with a row's largest
+    numerator weight held at 2^10 or more a weight is off by up to half of it,
+    2^-35 of the largest, so the sum by 2^-35 of the largest times the sum of
+    |v|.  (Over codes the numerator's weight is w_t s_t and the codes are at
+    most `top`: 2^-35 max(w_t s_t) n top <= 2^-35 n max|v|, the same.)"""
     half = torch.finfo(dtype).eps / 2
+    fixed = 0.0
     rel = 2 * (out.shape[-1] + 4) * 2.0 ** -24 * reach[..., None] + 2.0 ** -20
     if dtype != torch.float32:
-        rel = rel + 2.0 ** -12
+        rel = rel + 2.0 ** -11
+        fixed = 2.0 ** -35 * floor[..., None]
     tiny = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}
-    return half * out.abs() + (1 + half) * rel * spread + tiny[dtype]
+    return half * out.abs() + (1 + half) * (rel * spread + fixed) + tiny[dtype]
