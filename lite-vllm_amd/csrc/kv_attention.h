@@ -84,8 +84,9 @@ struct Call {
 struct TilePlan {
   int seq_begin, n_seqs, max_q;
   int rw;                   // tile kernel: 32-row groups of a unit, 1, 2 or 4; 0: narrow kernel
-  int grid;                 // workgroups, and ranges that the list is split into
-  int whole, slot_heads, slot_rows;
+  int grid, ranges;         // workgroups; ranges that the list is split into
+  int direct, nq;           // (see TileArgs)
+  int slot_heads, slot_rows;
   size_t head_bytes, ml_bytes, acc_bytes;
 };
 

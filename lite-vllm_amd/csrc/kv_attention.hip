@@ -200,23 +200,30 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   const int r = 32 * p.rw, kt = p.rw == 4 ? 64 : 128;
   const int64_t units = (int64_t)n_seqs * num_kv_heads * ((rows + r - 1) / r);
   const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_blocks * kBs + kt - 1) / kt);
-  // contexts of a few tiles: splitting them costs more than it gives
-  p.whole = tiles <= 4;
   const int64_t cus = device_cus();
-  p.grid = (int)(p.whole ? std::min<int64_t>(units, 1 << 20)
-                         : std::min<int64_t>(units * tiles, cus * (dtype == LV_F32 ? 1 : 2)));
+  p.nq = (int)((rows + r - 1) / r);
+  p.ranges = (int)std::min<int64_t>(units * tiles, cus * (dtype == LV_F32 ? 1 : 2));
+  p.grid = p.ranges;
+  const int64_t all = ((int64_t)n_seqs * num_kv_heads + kXcds - 1) / kXcds * kXcds * p.nq;
+  if (all < (1ll << 31)) {
+    // contexts of a few tiles are not split; where there are half as many
+    // units again as run at once, the kernel looks whether they need to be
+    p.direct = tiles <= 4 ? 2 : 2 * units >= 3 * p.ranges ? 1 : 0;
+    if (p.direct) p.grid = (int)std::max<int64_t>(all, p.direct == 1 ? p.ranges : 0);
+  }
   p.slot_heads = 1;
   p.slot_rows = (int)std::min<int64_t>(rows, r);
-  if (codes && dtype != LV_F32 && rows <= 8 && !p.whole) {
+  if (codes && dtype != LV_F32 && rows <= 8 && p.direct != 2) {
     p.rw = 0;
+    p.direct = 0;
     p.slot_heads = std::min(num_kv_heads, 8);
     while (num_kv_heads % p.slot_heads != 0) --p.slot_heads;
     const int64_t list = (int64_t)n_seqs * (num_kv_heads / p.slot_heads) * ((max_blocks + 1) / 2);
-    p.grid = (int)std::min<int64_t>(list, cus * (8 / p.slot_heads));
+    p.grid = p.ranges = (int)std::min<int64_t>(list, cus * (8 / p.slot_heads));
   }
-  if (!p.whole) {
-    const size_t slots = (size_t)2 * p.grid * p.slot_heads * p.slot_rows;
-    p.head_bytes = align256((size_t)p.grid * 2 * 16);
+  if (p.direct != 2) {
+    const size_t slots = (size_t)2 * p.ranges * p.slot_heads * p.slot_rows;
+    p.head_bytes = align256((size_t)p.ranges * 2 * 16);
     p.ml_bytes = align256(slots * 8);
     p.acc_bytes = align256(slots * head_dim * 4);
   }

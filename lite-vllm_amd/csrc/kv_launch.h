@@ -10,7 +10,9 @@ inline TileArgs tile_args(const Call& a, const TilePlan& p, char* ws) {
   TileArgs t{};
   t.b = a.b; t.c = a.c; t.r = a.r;
   t.seq_begin = p.seq_begin; t.n_seqs = p.n_seqs; t.max_q = p.max_q;
-  t.whole = p.whole;
+  t.ranges = p.ranges;
+  t.direct = p.direct;
+  t.nq = p.nq;
   t.slot_heads = p.slot_heads;
   t.slot_rows = p.slot_rows;
   t.head = reinterpret_cast<int4*>(ws);
@@ -25,7 +27,7 @@ int launch_join(const Call& a, const TilePlan& p, const TileArgs& t) {
   // few rows may have many pieces: the teams share them
   const int rows = p.slot_heads * p.slot_rows;
   const int rows_per = p.slot_rows <= 8 ? 1 : TEAMS;
-  attn_join_kernel<T, D><<<dim3((unsigned)p.grid - 1, (unsigned)((rows + rows_per - 1) / rows_per)),
+  attn_join_kernel<T, D><<<dim3((unsigned)p.ranges - 1, (unsigned)((rows + rows_per - 1) / rows_per)),
                            256, 0, a.stream>>>(t, rows_per);
   return check_launch("attn_join_kernel");
 }
@@ -36,7 +38,7 @@ int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
   const TileArgs t = tile_args(a, p, ws);
   const size_t lds = F::lds(D) + (size_t)(p.n_seqs + 1) * 4;
   attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, kTileThreads, lds, a.stream>>>(t);
-  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.whole || p.grid < 2)
+  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct == 2 || p.ranges < 2)
     return rc;
   return launch_join<T, D>(a, p, t);
 }

@@ -17,7 +17,10 @@ namespace lv {
 // unlike the contexts are, and nothing about them has to be known on the
 // host.  A unit inside one range is written to `out`; the pieces of one that
 // spans several go to the workspace (m, l, O / l in fp32) and attn_join_kernel
-// joins them.
+// joins them.  Where there are many units and none is long against a range, a
+// workgroup takes a whole unit instead (direct), longest sequences and last
+// rows first, so that there are no pieces: 15 chunks of 512 tokens at offsets
+// of 0-3071 (960 units) beside 192 decode rows 398 -> 369 us.
 //
 // A workgroup is 4 wavefronts: RW groups of 32 rows times KW = 4 / RW parts
 // of every tile's keys, so that few rows (RW = 1: decodes, small trees) still
@@ -54,7 +57,9 @@ constexpr int kTileThreads = 256;
 struct TileArgs {
   Batch b; KvView c; Rows r;
   int seq_begin, n_seqs, max_q;
-  int whole;                // ranges of whole units: nothing to join
+  int ranges;               // ranges of the list
+  int direct;               // a workgroup per unit: 2 always, 1 if no unit is long
+  int nq;                   // row tiles of a unit's sequence, at most
   int slot_heads, slot_rows;   // kv heads of a workspace slot, rows of each
   int4* head;               // [ranges][2]: the unit that crosses a range's start
   float* ml;                // [2 ranges][slot_heads][slot_rows][2]
@@ -65,6 +70,15 @@ struct Unit {
   int seq, q0, n, rows, committed, kend, kvh, row0, ntiles;
   int unit2;     // the V scales' unit is 2^unit2 (16-bit queries over codes)
 };
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// The same in all lanes: said to the compiler, which does not see it of what
+// comes out of LDS, so that all that follows from a unit is scalar.
+__device__ __forceinline__ void make_uniform(Unit& u) {
+  u.seq = uniform(u.seq); u.q0 = uniform(u.q0); u.n = uniform(u.n); u.rows = uniform(u.rows);
+  u.committed = uniform(u.committed); u.kend = uniform(u.kend); u.kvh = uniform(u.kvh);
+  u.row0 = uniform(u.row0); u.ntiles = uniform(u.ntiles);
+}
 
 template <int RW> struct TileCfg {
   static constexpr int R = 32 * RW, KW = 4 / RW;
@@ -90,13 +104,12 @@ __device__ __forceinline__ Seq tile_sequence(const TileArgs& a, int i) {
 
 // Tiles of sequence i, over all its row tiles and kv heads.
 template <bool TREE, int RW>
-__device__ __forceinline__ int sequence_tiles(const TileArgs& a, int i, int g) {
+__device__ __forceinline__ int sequence_tiles(const TileArgs& a, const Seq& s, int g) {
   using F = TileCfg<RW>;
-  const Seq s = tile_sequence(a, i);
   const int rows = min(s.n, a.max_q) * g;
   int sum = 0;
-  if (TREE || a.whole) {
-    sum = (rows + F::R - 1) / F::R * (a.whole ? 1 : max(1, (s.ctx + F::KT - 1) / F::KT));
+  if (TREE) {
+    sum = (rows + F::R - 1) / F::R * max(1, (s.ctx + F::KT - 1) / F::KT);
   } else {
     for (int r0 = 0; r0 < rows; r0 += F::R)
       sum += max(1, (keys_needed<TREE, F::R>(s.ctx, s.ctx - s.n, rows, r0, g) + F::KT - 1) / F::KT);
@@ -104,17 +117,22 @@ __device__ __forceinline__ int sequence_tiles(const TileArgs& a, int i, int g) {
   return sum * a.r.num_kv_heads;
 }
 
-// Exclusive scan of the sequences' tiles into off[0 .. n_seqs].
+// Exclusive scan of the sequences' tiles into off[0 .. n_seqs]; returns the
+// longest unit's tiles.
 template <bool TREE, int RW>
-__device__ void scan_tiles(const TileArgs& a, int g, int* off, int* part) {
+__device__ int scan_tiles(const TileArgs& a, int g, int* off, int* part) {
+  using F = TileCfg<RW>;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.n_seqs + kTileThreads - 1) / kTileThreads;
   const int lo = min(a.n_seqs, t * per), hi = min(a.n_seqs, lo + per);
-  int sum = 0;
+  int sum = 0, longest = 0;
   for (int i = lo; i < hi; ++i) {
     off[i] = sum;                       // within the thread's run
-    sum += sequence_tiles<TREE, RW>(a, i, g);
+    const Seq s = tile_sequence(a, i);
+    sum += sequence_tiles<TREE, RW>(a, s, g);
+    if (s.n > 0) longest = max(longest, (s.ctx + F::KT - 1) / F::KT);
   }
+  longest = (int)group_umax<64>((uint32_t)longest);
   int incl = sum;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -122,12 +140,31 @@ __device__ void scan_tiles(const TileArgs& a, int g, int* off, int* part) {
     if (lane >= d) incl += u;
   }
   if (lane == 63) part[wave] = incl;
+  if (lane == 0) part[4 + wave] = longest;
   __syncthreads();
   int base = incl - sum;
   for (int w = 0; w < wave; ++w) base += part[w];
   for (int i = lo; i < hi; ++i) off[i] += base;
   if (t == kTileThreads - 1) off[a.n_seqs] = base + sum;
+  for (int w = 0; w < 4; ++w) longest = max(longest, part[4 + w]);
   __syncthreads();
+  return longest;
+}
+
+// The sequence that direct workgroups of rank r take: the r-th by descending
+// context (ties by index) where they are few enough to rank, r otherwise.
+constexpr int kRankMax = kTileThreads;
+__device__ __forceinline__ int ranked_sequence(const TileArgs& a, int r, int* ctx, int* pick) {
+  if (a.n_seqs > kRankMax) return r;
+  const int t = threadIdx.x;
+  const int mine = t < a.n_seqs ? tile_sequence(a, t).ctx : -1;
+  ctx[t] = mine;
+  __syncthreads();
+  int before = 0;
+  for (int i = 0; i < a.n_seqs; ++i) before += ctx[i] > mine || (ctx[i] == mine && i < t);
+  if (t < a.n_seqs && before == r) *pick = t;
+  __syncthreads();
+  return *pick;
 }
 
 template <bool TREE, int RW>
@@ -160,11 +197,10 @@ __device__ __forceinline__ int locate(const TileArgs& a, const int* off, int p, 
   rem -= u.kvh * per_head;
   for (u.row0 = 0;; u.row0 += F::R) {
     set_rows<TREE, RW>(a, u, ctx, g);
-    const int c = a.whole ? 1 : u.ntiles;
-    if (rem < c || u.row0 + F::R >= u.rows) break;
-    rem -= c;
+    if (rem < u.ntiles || u.row0 + F::R >= u.rows) break;
+    rem -= u.ntiles;
   }
-  return a.whole ? 0 : rem;
+  return rem;
 }
 
 template <bool TREE, int RW>
@@ -300,37 +336,57 @@ void attn_tile_kernel(TileArgs a) {
   float* const s_sc = reinterpret_cast<float*>(s_kv + NST * 2 * TILE);
   float2* const s_ml = reinterpret_cast<float2*>(s_sc + NST * 3 * KT);   // [4][32]
   int* const s_off = reinterpret_cast<int*>(s_ml + 128);
-  __shared__ int s_part[4];
+  __shared__ int s_part[8], s_ctx[kRankMax], s_pick;
 
   const int H = a.r.num_heads, Hkv = a.r.num_kv_heads;
   const int G = H / Hkv;
-  scan_tiles<TREE, RW>(a, G, s_off, s_part);
-  const int total = s_off[a.n_seqs];
-  const int grid = (int)gridDim.x;
-  // neighbouring ranges on one XCD: they read the same cached rows
-  const int w = grid % kXcds == 0 ? (int)(blockIdx.x % kXcds) * (grid / kXcds) +
-                                        (int)(blockIdx.x / kXcds)
-                                  : (int)blockIdx.x;
-  const int per = max(1, (int)(((int64_t)total + grid - 1) / grid));
-  const int r0 = (int)min((int64_t)total, (int64_t)w * per);
-  const int r1 = (int)min((int64_t)total, (int64_t)(w + 1) * per);
-  if (!a.whole && threadIdx.x == 0) a.head[2 * w] = make_int4(0, 0, 0, 0);
-  if (r0 >= r1) return;
-
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rg = wave % RW, kg = wave / RW;
   const int lr = lane & 31, h = lane >> 5;
 
+  int r0 = 0, r1 = 1, w = 0, t = 0, per = 1;
+  bool direct = a.direct == 2;
+  if (!direct) {
+    const int longest = uniform(scan_tiles<TREE, RW>(a, G, s_off, s_part));
+    const int total = uniform(s_off[a.n_seqs]);
+    per = max(1, (int)(((int64_t)total + a.ranges - 1) / a.ranges));
+    direct = a.direct == 1 && longest <= 2 * per;
+    const int b = (int)blockIdx.x;
+    // neighbouring ranges on one XCD: they read the same cached rows
+    w = a.ranges % kXcds == 0 ? b % kXcds * (a.ranges / kXcds) + b / kXcds : b;
+    if (b < a.ranges && threadIdx.x == 0) a.head[2 * w] = make_int4(0, 0, 0, 0);
+    if (!direct) {
+      if (b >= a.ranges) return;
+      r0 = (int)min((int64_t)total, (int64_t)w * per);
+      r1 = (int)min((int64_t)total, (int64_t)(w + 1) * per);
+      if (r0 >= r1) return;
+    }
+  }
   Unit U;
-  int t = locate<TREE, RW>(a, s_off, r0, G, U);
-  if (!a.whole && t > 0 && threadIdx.x == 0) {
-    // the range starts inside a unit; if that unit starts in the range
-    // before, this range's workgroup of the join takes it
-    const int start = r0 - t, end = start + U.ntiles;
-    if (start >= r0 - per) {
-      a.head[2 * w] = make_int4((end - 1) / per - w + 2, U.q0, U.kvh, U.row0);
-      a.head[2 * w + 1] = make_int4(min(F::R, U.rows - U.row0), 0, 0, 0);
+  if (direct) {
+    // all row tiles of a (sequence, kv head) on one XCD
+    const int slot = (int)blockIdx.x / kXcds;
+    const int grp = slot / a.nq * kXcds + (int)blockIdx.x % kXcds;
+    if (grp >= a.n_seqs * Hkv) return;
+    const int seq = uniform(ranked_sequence(a, grp / Hkv, s_ctx, &s_pick));
+    const int ctx = set_seq(a, U, seq, G);
+    U.kvh = grp % Hkv;
+    U.row0 = (a.nq - 1 - slot % a.nq) * F::R;
+    if (U.row0 >= U.rows) return;
+    set_rows<TREE, RW>(a, U, ctx, G);
+    make_uniform(U);
+  } else {
+    t = uniform(locate<TREE, RW>(a, s_off, r0, G, U));
+    make_uniform(U);
+    if (t > 0 && threadIdx.x == 0) {
+      // the range starts inside a unit; if that unit starts in the range
+      // before, this range's workgroup of the join takes it
+      const int start = r0 - t, end = start + U.ntiles;
+      if (start >= r0 - per) {
+        a.head[2 * w] = make_int4((end - 1) / per - w + 2, U.q0, U.kvh, U.row0);
+        a.head[2 * w + 1] = make_int4(min(F::R, U.rows - U.row0), 0, 0, 0);
+      }
     }
   }
 
@@ -362,8 +418,8 @@ void attn_tile_kernel(TileArgs a) {
           v = a.c.scale[1][phys * a.c.sblk + (key % kBs) * a.c.stok + u.kvh * a.c.shead];
         }
         v = group_max<64>(v > 0.0f && v < __builtin_inff() ? v : 0.0f);
-        const int e = (int)(__builtin_amdgcn_readfirstlane(__float_as_uint(v)) >> 23) - 127;
-        u.unit2 = v > 0.0f ? min(max(e, -100), 100) : 0;
+        const int e = uniform((int)(__float_as_uint(v) >> 23));      // 0: no scale
+        u.unit2 = e > 0 ? min(max(e - 127, -100), 100) : 0;
       }
     }
     int phys[BPW];     // (read by all lanes: a readlane under a branch sees stale copies)
@@ -804,15 +860,16 @@ void attn_tile_kernel(TileArgs a) {
   // The tile after (u, tile) at place p of the list: true if there is one;
   // `inside`: it belongs to the same unit.
   auto advance = [&](Unit& u, int& tile, int& p, bool& inside) {
-    inside = tile + 1 < u.ntiles && (a.whole || p + 1 < r1);
+    inside = tile + 1 < u.ntiles && (direct || p + 1 < r1);
     if (inside) {
       ++tile;
-      p += a.whole ? 0 : 1;
+      p += direct ? 0 : 1;
       return true;
     }
     if (p + 1 >= r1) return false;
     ++p;
     u = next_unit<TREE, RW>(a, u, G);
+    make_uniform(u);
     tile = 0;
     return true;
   };
