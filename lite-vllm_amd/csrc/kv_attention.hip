@@ -204,16 +204,18 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   p.nq = (int)((rows + r - 1) / r);
   p.ranges = (int)std::min<int64_t>(units * tiles, cus * (dtype == LV_F32 ? 1 : 2));
   p.grid = p.ranges;
+  const bool one_round = units <= cus * (dtype == LV_F32 ? 1 : 2);
   const int64_t all = ((int64_t)n_seqs * num_kv_heads + kXcds - 1) / kXcds * kXcds * p.nq;
   if (all < (1ll << 31)) {
-    // contexts of a few tiles are not split; where there are half as many
+    // contexts of a few tiles are not split where all units run at once (a
+    // join takes as long as two tiles or three); where there are half as many
     // units again as run at once, the kernel looks whether they need to be
-    p.direct = tiles <= 4 ? 2 : 2 * units >= 3 * p.ranges ? 1 : 0;
+    p.direct = tiles <= (one_round ? 4 : 2) ? 2 : 2 * units >= 3 * p.ranges ? 1 : 0;
     if (p.direct) p.grid = (int)std::max<int64_t>(all, p.direct == 1 ? p.ranges : 0);
   }
   p.slot_heads = 1;
   p.slot_rows = (int)std::min<int64_t>(rows, r);
-  if (codes && dtype != LV_F32 && rows <= 8 && p.direct != 2) {
+  if (codes && dtype != LV_F32 && rows <= 8 && !(p.direct == 2 && one_round)) {
     p.rw = 0;
     p.direct = 0;
     p.slot_heads = std::min(num_kv_heads, 8);

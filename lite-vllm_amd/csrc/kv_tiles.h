@@ -265,7 +265,8 @@ __device__ __forceinline__ uint32_t take_part(float& a, float& b, bool last) {
     b -= __uint_as_float(w & 0xffff0000u);
     return w;
   } else {
-    const uint32_t w = Mfma32<f16>::pack2(a, b);
+    const uint32_t w = __builtin_bit_cast(
+        uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));     // one instruction
     if (!last) {
       a -= f16_bits_to_float(w & 0xffffu);
       b -= f16_bits_to_float(w >> 16);

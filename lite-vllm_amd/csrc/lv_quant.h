@@ -69,6 +69,11 @@ __device__ __forceinline__ uint32_t group_umax(uint32_t x) {
 // Scale of a row and its N values x of this lane divided by it (zeros where
 // the scale is 0 or NaN), the row spread over W lanes.  Magnitudes are
 // compared as bits, which keeps NaN the largest of all.
+// The quotients are the correctly rounded ones: x r, r the correctly rounded
+// reciprocal, corrected once by its exact remainder (Markstein's division; the
+// scales outside the range where no step of it underflows are divided).  Three
+// instructions instead of ten for each value, which bounded the writers: 7872
+// tokens of 8 heads of 128 bf16 dims 17.7 -> 15.8 us.
 template <typename C, int W, int N>
 __device__ __forceinline__ float row_scale(float* x) {
   uint32_t top = 0;
@@ -77,9 +82,18 @@ __device__ __forceinline__ float row_scale(float* x) {
   top = group_umax<W>(top);
   const float scale = top >= 0x7f800000u ? __builtin_nanf("")
                                          : __uint_as_float(top) / code<C>::kTop;
-  const bool live = scale > 0.0f;
+  if (scale >= 0x1p-80f && scale <= 0x1p100f) {
+    const float r = 1.0f / scale;
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = live ? x[i] / scale : 0.0f;
+    for (int i = 0; i < N; ++i) {
+      const float q = x[i] * r;
+      x[i] = fmaf(fmaf(-q, scale, x[i]), r, q);
+    }
+  } else {
+    const bool live = scale > 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = live ? x[i] / scale : 0.0f;
+  }
   return scale;
 }
 
