@@ -5,7 +5,8 @@ Field names and defaults follow the reference's config/config.py:15-178
 user code carries over.  Additions: ``SamplingParams.ignore_eos`` (the
 reference has none; its EOS falls back to token 0, tokenizer.py:48-51),
 ``ModelConfig.load_format="dummy"`` (seeded random weights, no checkpoint)
-and ``ModelConfig.from_hf_dict`` for architectures given as a plain dict.
+and ``ModelConfig.from_hf_dict`` for architectures given as a plain dict;
+``CacheConfig.kv_cache_dtype``, an 8-bit K/V cache.
 """
 
 from __future__ import annotations
@@ -93,9 +94,16 @@ class CacheConfig:
     num_cpu_blocks: int = 0
     gpu_memory_utilization: float = 0.85
     enable_prefix_caching: bool = False
+    # "auto": the model's dtype; "int8" / "fp8": 8-bit codes with a scale per
+    # token and kv head (half the memory and the decode steps' reads)
+    kv_cache_dtype: str = "auto"
     # decode rows whose block tables start with the same blocks read that
-    # shared prefix once per group in attention
+    # shared prefix once per group in attention (16-bit caches)
     shared_prefix_attention: bool = True
+
+    def __post_init__(self) -> None:
+        if self.kv_cache_dtype not in ("auto", "int8", "fp8"):
+            raise ValueError('kv_cache_dtype must be "auto", "int8" or "fp8"')
 
 
 @dataclass

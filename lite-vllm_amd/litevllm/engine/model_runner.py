@@ -350,18 +350,24 @@ class DecodeGraphs:
             "context_lens": torch.zeros(n, dtype=torch.int32, device=dev),
             "block_tables": torch.zeros((n, self.max_blocks), dtype=torch.int32, device=dev),
         }
-        ws = max(ops.paged_attention_workspace_size(b, b, b, mc.num_attention_heads, mc.head_dim,
-                                                    cc.block_size, self.max_blocks, 1,
-                                                    mc.torch_dtype) for b in self.batches)
+        if cc.kv_cache_dtype != "auto":
+            ws = max(ops.paged_attention_quant_workspace_size(
+                b, b, b, 1, mc.num_attention_heads, mc.num_key_value_heads, mc.head_dim,
+                self.max_blocks, mc.torch_dtype) for b in self.batches)
+        else:
+            ws = max(ops.paged_attention_workspace_size(
+                b, b, b, mc.num_attention_heads, mc.head_dim, cc.block_size, self.max_blocks, 1,
+                mc.torch_dtype) for b in self.batches)
         self.workspace = torch.empty(max(ws, 256), dtype=torch.uint8, device=dev)
         # Shared-prefix plan, one static int32 buffer: blocks [n] (padded to
         # a multiple of 4 so the items stay 16-byte aligned), items
         # [PREFIX_MAX_ITEMS, 4], members [n].  Every graph reads all of it;
         # rows and items beyond a graph's batch are skipped by the kernel.
         self.group_size = mc.num_attention_heads // mc.num_key_value_heads
-        self.use_prefix = cc.shared_prefix_attention and ops.prefix_attention_supported(
-            mc.num_attention_heads, mc.num_key_value_heads, mc.head_dim, cc.block_size,
-            mc.torch_dtype)
+        self.use_prefix = (cc.shared_prefix_attention and cc.kv_cache_dtype == "auto"
+                           and ops.prefix_attention_supported(
+                               mc.num_attention_heads, mc.num_key_value_heads, mc.head_dim,
+                               cc.block_size, mc.torch_dtype))
         self._pfx_active = False
         if self.use_prefix:
             npad = (n + 3) // 4 * 4
@@ -525,7 +531,8 @@ class ModelRunner:
         mc = self.model_config
         self.kv_cache = KVCache(mc.num_hidden_layers, num_gpu_blocks,
                                 self.config.cache_config.block_size, mc.num_key_value_heads,
-                                mc.head_dim, mc.torch_dtype, self.device)
+                                mc.head_dim, mc.torch_dtype, self.device,
+                                self.config.cache_config.kv_cache_dtype)
 
     def profile_num_gpu_blocks(self) -> int:
         """KV blocks fitting in gpu_memory_utilization of the device memory
@@ -542,7 +549,8 @@ class ModelRunner:
         available = int(total * self.config.cache_config.gpu_memory_utilization) - used
         n = KVCache.profile_num_blocks(available, mc.num_hidden_layers,
                                        self.config.cache_config.block_size,
-                                       mc.num_key_value_heads, mc.head_dim, mc.torch_dtype)
+                                       mc.num_key_value_heads, mc.head_dim, mc.torch_dtype,
+                                       self.config.cache_config.kv_cache_dtype)
         return max(n, 16)
 
     def capture_decode_graphs(self) -> None:
@@ -624,6 +632,8 @@ class ModelRunner:
         cc = self.config.cache_config
         mc = self.model_config
         if not cc.shared_prefix_attention or not 2 <= st.num_decodes <= ops.PREFIX_MAX_DECODES:
+            return None
+        if cc.kv_cache_dtype != "auto":
             return None
         if not ops.prefix_attention_supported(mc.num_attention_heads, mc.num_key_value_heads,
                                               mc.head_dim, cc.block_size, mc.torch_dtype):

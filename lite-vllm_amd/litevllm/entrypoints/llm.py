@@ -3,7 +3,8 @@
 Same constructor knobs and generate() contract (outputs in completion
 order, greedy max_tokens=256 by default); additions: prompt_token_ids for
 tokenizer-free use, load_format="dummy" / hf_overrides for seeded random
-weights of a given architecture, skip_tokenizer_init.
+weights of a given architecture, skip_tokenizer_init, kv_cache_dtype="int8" or
+"fp8" for an 8-bit K/V cache.
 """
 
 from __future__ import annotations
@@ -24,14 +25,16 @@ class LLM:
                  chunk_size: int = 512, trust_remote_code: bool = True, seed: int = 0,
                  load_format: str = "auto", hf_overrides: Optional[dict] = None,
                  skip_tokenizer_init: bool = False, num_gpu_blocks: Optional[int] = None,
-                 device: str = "auto", enforce_eager: bool = False) -> None:
+                 device: str = "auto", enforce_eager: bool = False,
+                 kv_cache_dtype: str = "auto") -> None:
         cfg = EngineConfig(
             model_config=ModelConfig(model=model, dtype=dtype, max_model_len=max_model_len,
                                      trust_remote_code=trust_remote_code,
                                      load_format=load_format, hf_overrides=hf_overrides),
             cache_config=CacheConfig(block_size=block_size, num_gpu_blocks=num_gpu_blocks,
                                      gpu_memory_utilization=gpu_memory_utilization,
-                                     enable_prefix_caching=enable_prefix_caching),
+                                     enable_prefix_caching=enable_prefix_caching,
+                                     kv_cache_dtype=kv_cache_dtype),
             scheduler_config=SchedulerConfig(max_num_seqs=max_num_seqs,
                                              max_num_batched_tokens=max_num_batched_tokens,
                                              chunked_prefill=chunked_prefill,
@@ -71,10 +74,12 @@ def main() -> None:
     parser.add_argument("--top-k", type=int, default=-1)
     parser.add_argument("--dtype", type=str, default="auto")
     parser.add_argument("--seed", type=int, default=0)
+    parser.add_argument("--kv-cache-dtype", choices=["auto", "int8", "fp8"], default="auto")
     args = parser.parse_args()
     params = SamplingParams(temperature=args.temperature, top_p=args.top_p, top_k=args.top_k,
                             max_tokens=args.max_tokens)
-    llm = LLM(model=args.model, dtype=args.dtype, seed=args.seed)
+    llm = LLM(model=args.model, dtype=args.dtype, seed=args.seed,
+              kv_cache_dtype=args.kv_cache_dtype)
     for out in llm.generate([args.prompt], params):
         print(f"\nPrompt: {out.prompt_text}\nOutput: {out.output_text}\n"
               f"Tokens: {out.num_prompt_tokens} prompt + {out.num_output_tokens} generated")

@@ -8,7 +8,9 @@ either causal attention over this forward's own tokens (prefill,
 attention.py:141-151) or paged decode over the block tables (91-139).  The
 engine passes ``attn_metadata`` instead, describing a mixed batch (decodes
 first, then prefill chunks at any offset) that one lv_paged_attention call
-serves.
+serves.  With ``attn_metadata.tree_mask`` the rows are trees of drafted tokens
+instead.  ``key_cache`` may be an 8-bit cache (ops.QuantKV, ``value_cache``
+then None).
 """
 
 from __future__ import annotations
@@ -35,14 +37,20 @@ class AttentionMetadata:
     # decode rows' shared prefixes, read once per group (lv_paged_attention_prefix)
     prefix: Optional[ops.PrefixPlan] = None
     prefix_workspace: Optional[torch.Tensor] = None
+    # int64 [T, words]: the rows are drafted token trees (ops.tree_mask)
+    tree_mask: Optional[torch.Tensor] = None
 
 
 class PagedAttention:
     @staticmethod
     def write_to_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor,
                        value_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
-        """key_cache[slot // bs, slot % bs] = key (reference attention.py:17-33)."""
-        ops.kv_scatter(key, value, key_cache, value_cache, slot_mapping)
+        """key_cache[slot // bs, slot % bs] = key (reference attention.py:17-33);
+        key_cache may be an 8-bit cache."""
+        if isinstance(key_cache, ops.QuantKV):
+            ops.kv_scatter_quant(key, value, key_cache, slot_mapping)
+        else:
+            ops.kv_scatter(key, value, key_cache, value_cache, slot_mapping)
 
 
 class Attention(nn.Module):
@@ -58,9 +66,16 @@ class Attention(nn.Module):
     def forward(self, query, key, value, key_cache, value_cache, block_table, slot_mapping,
                 context_lens, is_prefill=True, attn_metadata: Optional[AttentionMetadata] = None):
         if slot_mapping is not None and key_cache is not None:
-            ops.kv_scatter(key, value, key_cache, value_cache, slot_mapping)
+            PagedAttention.write_to_cache(key, value, key_cache, value_cache, slot_mapping)
+        if isinstance(key_cache, ops.QuantKV) and (attn_metadata is not None or not is_prefill):
+            return self._quant(query, key_cache, block_table, context_lens, attn_metadata)
         if attn_metadata is not None:
             m = attn_metadata
+            if m.tree_mask is not None:
+                return ops.tree_attention(query, key_cache, value_cache, m.block_tables,
+                                          m.context_lens, m.cu_seqlens, m.tree_mask,
+                                          scale=self.scale, max_query_len=m.max_query_len,
+                                          workspace=m.workspace)
             return ops.paged_attention(query, key_cache, value_cache, m.block_tables,
                                        m.context_lens, scale=self.scale, cu_seqlens=m.cu_seqlens,
                                        num_decodes=m.num_decodes, max_query_len=m.max_query_len,
@@ -70,6 +85,19 @@ class Attention(nn.Module):
             return self._prefill(query, key, value)
         return ops.paged_attention(query, key_cache, value_cache, block_table, context_lens,
                                    scale=self.scale)
+
+    def _quant(self, query, cache, block_table, context_lens, m: Optional[AttentionMetadata]):
+        if m is None:
+            return ops.paged_attention_quant(query, cache, block_table, context_lens,
+                                             scale=self.scale)
+        if m.tree_mask is not None:
+            return ops.tree_attention_quant(query, cache, m.block_tables, m.context_lens,
+                                            m.cu_seqlens, m.tree_mask, scale=self.scale,
+                                            max_query_len=m.max_query_len, workspace=m.workspace)
+        return ops.paged_attention_quant(query, cache, m.block_tables, m.context_lens,
+                                         scale=self.scale, cu_seqlens=m.cu_seqlens,
+                                         num_decodes=m.num_decodes,
+                                         max_query_len=m.max_query_len, workspace=m.workspace)
 
     def _prefill(self, query, key, value):
         """Causal attention over this forward's T tokens only (one sequence at

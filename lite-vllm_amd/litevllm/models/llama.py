@@ -158,14 +158,18 @@ class DecoderAttention(nn.Module):
         if attn_metadata is not None and kv_cache is not None:
             # engine path: one fused prologue kernel (q/k norm, RoPE, K/V into
             # the paged cache), then attention over the cache
-            key_cache, value_cache = kv_cache
-            q = ops.qk_norm_rope_cache(
-                qkv, self.num_heads, self.num_kv_heads, self.head_dim,
-                self.rotary_emb.cos_cached, self.rotary_emb.sin_cached, positions, slot_mapping,
-                key_cache, value_cache,
-                q_norm_weight=self.q_norm.weight if self.use_qk_norm else None,
-                k_norm_weight=self.k_norm.weight if self.use_qk_norm else None,
-                eps=self.q_norm.eps if self.use_qk_norm else 1e-6)
+            norms = dict(q_norm_weight=self.q_norm.weight if self.use_qk_norm else None,
+                         k_norm_weight=self.k_norm.weight if self.use_qk_norm else None,
+                         eps=self.q_norm.eps if self.use_qk_norm else 1e-6)
+            args = (qkv, self.num_heads, self.num_kv_heads, self.head_dim,
+                    self.rotary_emb.cos_cached, self.rotary_emb.sin_cached, positions,
+                    slot_mapping)
+            if isinstance(kv_cache, ops.QuantKV):
+                key_cache, value_cache = kv_cache, None
+                q = ops.qk_norm_rope_cache_quant(*args, kv_cache, **norms)
+            else:
+                key_cache, value_cache = kv_cache
+                q = ops.qk_norm_rope_cache(*args, key_cache, value_cache, **norms)
             out = self.attn(q, None, None, key_cache, value_cache, block_table, None,
                             context_lens, is_prefill, attn_metadata=attn_metadata)
             return self.o_proj(out.reshape(T, self.q_size))
@@ -179,7 +183,10 @@ class DecoderAttention(nn.Module):
         cos, sin = self.rotary_emb(positions)
         q = apply_rotary_emb(q, cos.unsqueeze(1), sin.unsqueeze(1))
         k = apply_rotary_emb(k, cos.unsqueeze(1), sin.unsqueeze(1))
-        key_cache, value_cache = kv_cache if kv_cache is not None else (None, None)
+        if isinstance(kv_cache, ops.QuantKV):
+            key_cache, value_cache = kv_cache, None
+        else:
+            key_cache, value_cache = kv_cache if kv_cache is not None else (None, None)
         out = self.attn(q, k, v, key_cache, value_cache, block_table, slot_mapping, context_lens,
                         is_prefill, attn_metadata=attn_metadata)
         return self.o_proj(out.reshape(T, self.q_size))
