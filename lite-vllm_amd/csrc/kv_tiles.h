@@ -392,72 +392,79 @@ void attn_tile_kernel(TileArgs a) {
   }
 
   // -- loading -------------------------------------------------------------
+  // What follows from the unit alone is set once a piece (set_piece).
   uint4 kraw[BPW][LPB], vraw[BPW][LPB];
   float sraw = 0.0f;             // a scale (K of keys 0 .., then V) of the wavefront's blocks
-  int ids[BPW], id_first = 0, id_unit = -1;
+  int ids[BPW], id_first = 0;
+  const char *kbase = nullptr, *vbase = nullptr;
+  const float* sbase = nullptr;
   const int lrow = lane / CPR, lchunk = lane % CPR;
-  auto load_ids = [&](const Unit& u, int first) {
-    const int last = (u.kend - 1) / kBs;
+  int64_t loff[LPB];
+#pragma unroll
+  for (int i = 0; i < LPB; ++i)
+    loff[i] = (int64_t)(RPL * i + lrow) * a.c.tok * E::kBytes + 16 * lchunk;
+  auto load_ids = [&](int first) {
+    const int last = (U.kend - 1) / kBs;
 #pragma unroll
     for (int j = 0; j < BPW; ++j) {
       ids[j] = 0;
-      if (u.kend > 0)
-        ids[j] = physical_block(a.b, a.c.num_blocks, a.seq_begin + u.seq,
+      if (U.kend > 0)
+        ids[j] = physical_block(a.b, a.c.num_blocks, a.seq_begin + U.seq,
                                 min((first + lane) * (KT / kBs) + wave * BPW + j, last));
     }
     id_first = first;
   };
-  auto load_tile = [&](Unit& u, int tile, bool fresh) {
-    if (fresh || tile - id_first >= 64) load_ids(u, tile);
-    if constexpr (P::kLog) {
-      if (fresh) {       // the unit of the V scales: the largest of the first 64
-        float v = 0.0f;
-        const int key = tile * KT + lane;
-        if (key < u.kend) {
-          const int64_t phys =
-              physical_block(a.b, a.c.num_blocks, a.seq_begin + u.seq, key / kBs);
-          v = a.c.scale[1][phys * a.c.sblk + (key % kBs) * a.c.stok + u.kvh * a.c.shead];
-        }
-        v = group_max<64>(v > 0.0f && v < __builtin_inff() ? v : 0.0f);
-        const int e = uniform((int)(__float_as_uint(v) >> 23));      // 0: no scale
-        u.unit2 = e > 0 ? min(max(e - 127, -100), 100) : 0;
-      }
+  auto set_piece = [&](int first) {
+    kbase = (const char*)a.c.kv[0] + U.kvh * a.c.head * E::kBytes;
+    vbase = (const char*)a.c.kv[1] + U.kvh * a.c.head * E::kBytes;
+    load_ids(first);
+    if constexpr (kCodes) {
+      // lanes 0 .. 16 BPW - 1 the K scales, the next as many the V scales
+      const bool of_v = (lane / (16 * BPW)) & 1;
+      sbase = (of_v ? a.c.scale[1] : a.c.scale[0]) + (lane & 15) * a.c.stok + U.kvh * a.c.shead;
     }
+    if constexpr (P::kLog) {     // the unit of the V scales: the largest of the first 64
+      float v = 0.0f;
+      const int key = first * KT + lane;
+      if (key < U.kend) {
+        const int64_t phys = physical_block(a.b, a.c.num_blocks, a.seq_begin + U.seq, key / kBs);
+        v = a.c.scale[1][phys * a.c.sblk + (key % kBs) * a.c.stok + U.kvh * a.c.shead];
+      }
+      v = group_max<64>(v > 0.0f && v < __builtin_inff() ? v : 0.0f);
+      const int e = uniform((int)(__float_as_uint(v) >> 23));      // 0: no scale
+      U.unit2 = e > 0 ? min(max(e - 127, -100), 100) : 0;
+    }
+  };
+  auto load_tile = [&](int tile) {
+    if (tile - id_first >= 64) load_ids(tile);
     int phys[BPW];     // (read by all lanes: a readlane under a branch sees stale copies)
 #pragma unroll
     for (int j = 0; j < BPW; ++j) phys[j] = __builtin_amdgcn_readlane(ids[j], tile - id_first);
 #pragma unroll
     for (int j = 0; j < BPW; ++j) {
-      const int64_t at = (int64_t)phys[j] * a.c.blk + u.kvh * a.c.head;
-      const char* kp = (const char*)a.c.kv[0] + at * E::kBytes;
-      const char* vp = (const char*)a.c.kv[1] + at * E::kBytes;
+      const int64_t at = (int64_t)phys[j] * a.c.blk * E::kBytes;
 #pragma unroll
       for (int i = 0; i < LPB; ++i) {
-        const int64_t o = (int64_t)(RPL * i + lrow) * a.c.tok * E::kBytes + 16 * lchunk;
-        kraw[j][i] = load16(kp + o);
-        vraw[j][i] = load16(vp + o);
+        kraw[j][i] = load16(kbase + at + loff[i]);
+        vraw[j][i] = load16(vbase + at + loff[i]);
       }
     }
     if constexpr (kCodes) {
-      // lanes 0 .. 16 BPW - 1 the K scales, the next as many the V scales
-      const int key = lane % (16 * BPW);
-      const bool of_v = (lane / (16 * BPW)) & 1;
-      const int64_t block = key < 16 ? phys[0] : phys[BPW - 1];
-      const float* base = of_v ? a.c.scale[1] : a.c.scale[0];
-      sraw = base[block * a.c.sblk + (key & 15) * a.c.stok + u.kvh * a.c.shead];
+      const int block = lane & 16 ? phys[BPW - 1] : phys[0];
+      sraw = sbase[block * a.c.sblk];
     }
   };
-  auto write_tile = [&](const Unit& u, int tile, int st) {
+  auto write_tile = [&](int tile, int st) {
     uint16_t* const Ks = s_kv + st * 2 * TILE;
     uint16_t* const Vs = Ks + TILE;
     const int key0 = tile * KT + wave * 16 * BPW;
-    const bool tail = key0 + 16 * BPW > u.kend;
+    const bool tail = key0 + 16 * BPW > U.kend;
 #pragma unroll
     for (int j = 0; j < BPW; ++j)
 #pragma unroll
       for (int i = 0; i < LPB; ++i) {
         const int row = 16 * (wave * BPW + j) + RPL * i + lrow;    // of the tile
-        if (tail && tile * KT + row >= u.kend) vraw[j][i] = make_uint4(0, 0, 0, 0);
+        if (tail && tile * KT + row >= U.kend) vraw[j][i] = make_uint4(0, 0, 0, 0);
         uint4 ko[OPC], vo[OPC];
         if constexpr (kCodes) {
           codes_to_operands<typename P::K, C>(kraw[j][i], ko);
@@ -476,11 +483,11 @@ void attn_tile_kernel(TileArgs a) {
       const int key = lane % (16 * BPW), kv = lane / (16 * BPW);
       const int row = 16 * wave * BPW + key;
       float* const sc = s_sc + st * 3 * KT;
-      const bool in = tile * KT + row < u.kend;
+      const bool in = tile * KT + row < U.kend;
       if (kv == 0) sc[row] = sraw * a.r.scale_log2;
       if (kv == 1) {
         if constexpr (P::kLog) {
-          const float v = sraw * pow2(-u.unit2);
+          const float v = sraw * pow2(-U.unit2);
           const bool ok = v >= 0x1p-60f && v <= 0x1p20f;
           sc[KT + row] = !in ? 0.0f : ok ? __builtin_amdgcn_logf(v) : v == 0.0f ? -60.0f : 0.0f;
           sc[2 * KT + row] = !in ? 0.0f : ok ? __builtin_amdgcn_rcpf(v)
@@ -500,13 +507,13 @@ void attn_tile_kernel(TileArgs a) {
   int qrow = 0, qhead = 0, lim = 0;          // this lane's row, head and last key
   bool live = false;
 
-  auto start = [&](const Unit& u) {
-    const int idx = u.row0 + 32 * rg + lr;
-    live = idx < u.rows;
-    const int use = live ? idx : u.row0;
-    qrow = u.q0 + use / G;
-    qhead = u.kvh * G + use % G;
-    lim = TREE ? u.kend - 1 : min(u.committed + use / G, u.kend - 1);
+  auto start = [&]() {
+    const int idx = U.row0 + 32 * rg + lr;
+    live = idx < U.rows;
+    const int use = live ? idx : U.row0;
+    qrow = U.q0 + use / G;
+    qhead = U.kvh * G + use % G;
+    lim = TREE ? U.kend - 1 : min(U.committed + use / G, U.kend - 1);
     const T* qp = (const T*)a.r.q + (int64_t)qrow * a.r.q_stride + (int64_t)qhead * D + 8 * h;
     if constexpr (P::QP == 1) {
       uint4 raw[QSTEPS];
@@ -539,21 +546,14 @@ void attn_tile_kernel(TileArgs a) {
     l_run = 0.0f;
   };
 
-  int kx[QSTEPS];
+  // Byte offsets in a stage of this lane's operands: the swizzle is an XOR of
+  // the chunk, so the chunk of k-step s (dim block b) is one more XOR away.
+  const uint32_t k_at = 2 * (lr * D + 8 * (h ^ L::swz(lr)));      // ^ 32 s
+  uint32_t v_at[2];                                               // ^ 64 b
   {
-    const int y = h ^ L::swz(lr);
+    const int vrow = 4 * h + ((lane & 15) >> 2), dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
-    for (int s = 0; s < QSTEPS; ++s) kx[s] = lr * D + 8 * ((2 * s) ^ y);
-  }
-  int voff[DBLK][2];
-  {
-    const int vrow = 4 * h + ((lane & 15) >> 2);
-#pragma unroll
-    for (int b = 0; b < DBLK; ++b) {
-      const int dim = 32 * b + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      voff[b][0] = L::at(vrow, dim >> 3) + (dim & 7);
-      voff[b][1] = L::at(vrow + 8, dim >> 3) + (dim & 7);
-    }
+    for (int i = 0; i < 2; ++i) v_at[i] = 2 * (L::at(vrow + 8 * i, dim >> 3) + (dim & 7));
   }
 
   // Bits of the 32 drafted keys from t0 on that this lane's row sees; keys
@@ -568,19 +568,20 @@ void attn_tile_kernel(TileArgs a) {
     return (uint32_t)v;
   };
 
-  auto compute = [&](const Unit& u, int tile, int st) {
+  auto compute = [&](int tile, int st) {
     const int k0 = tile * KT + kg * KPW;           // this wavefront's first key
-    const uint16_t* kt = s_kv + st * 2 * TILE + kg * KPW * D;
-    const uint16_t* vt = kt + TILE;
+    const uint32_t kt = (uint32_t)(2 * (st * 2 * TILE + kg * KPW * D)), vt = kt + 2 * TILE;
     const float* const s_ks = s_sc + st * 3 * KT + kg * KPW;
     const float* const s_vs = s_ks + KT;
     // Four K operands in flight: read j + 4 goes out when product j has taken
     // its buffer (left to itself, the compiler waits out each read in turn).
     f32x16_t sv[KB];
+    __builtin_amdgcn_s_setprio(1);
     {
       constexpr int NJ = KB * QSTEPS;
       auto kread = [&](int j) __attribute__((always_inline)) {
-        return *reinterpret_cast<const uint4*>(kt + 32 * (j / QSTEPS) * D + kx[j % QSTEPS]);
+        return *reinterpret_cast<const uint4*>(
+            s_dyn + ((kt + k_at) ^ (32 * (j % QSTEPS))) + 64 * (j / QSTEPS) * D);
       };
       uint4 ka[4];
 #pragma unroll
@@ -597,6 +598,7 @@ void attn_tile_kernel(TileArgs a) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     // x in log2 units; the first key that some row may not see
     float mx = kNegBig;
 #pragma unroll
@@ -618,13 +620,13 @@ void attn_tile_kernel(TileArgs a) {
         for (int i = 0; i < 16; ++i) sv[kb][i] *= a.r.scale_log2;
       }
     }
-    const int open = TREE ? u.committed : u.committed + u.row0 / G + 1;
-    if (k0 + KPW > min(open, u.kend)) {            // the same in all lanes
+    const int open = TREE ? U.committed : U.committed + U.row0 / G + 1;
+    if (k0 + KPW > min(open, U.kend)) {            // the same in all lanes
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const int kk = k0 + 32 * kb;
         uint32_t win = ~0u;
-        if constexpr (TREE) win = tree_window(kk - u.committed);
+        if constexpr (TREE) win = tree_window(kk - U.committed);
         const int d = lim - kk - 4 * h;
         win >>= 4 * h;
 #pragma unroll
@@ -651,6 +653,16 @@ void attn_tile_kernel(TileArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[b][i] *= alpha;
     }
+    i16x4_t vlo[2][DBLK], vhi[2][DBLK];
+    auto vread = [&](int buf, int step) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < DBLK; ++b) {
+        vlo[buf][b] = lds_read_tr16(reinterpret_cast<const uint16_t*>(
+            s_dyn + ((vt + v_at[0]) ^ (64 * b)) + 32 * step * D));
+        vhi[buf][b] = lds_read_tr16(reinterpret_cast<const uint16_t*>(
+            s_dyn + ((vt + v_at[1]) ^ (64 * b)) + 32 * step * D));
+      }
+    };
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -686,22 +698,18 @@ void attn_tile_kernel(TileArgs a) {
           sv[kb][2 * i] = x;
           sv[kb][2 * i + 1] = y;
         }
+      // Each step's V operands are read while the step before is multiplied.
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const uint16_t* vb = vt + (32 * kb + 16 * s) * D;
-        i16x4_t lo[DBLK], hi[DBLK];
-#pragma unroll
-        for (int b = 0; b < DBLK; ++b) {
-          lo[b] = lds_read_tr16(vb + voff[b][0]);
-          hi[b] = lds_read_tr16(vb + voff[b][1]);
-        }
+        if (kb == 0 && s == 0) vread(0, 0);
+        if (2 * kb + s + 1 < 2 * KB) vread((s + 1) & 1, 2 * kb + s + 1);
 #pragma unroll
         for (int p = P::PP - 1; p >= 0; --p) {
           const uint32_t* pp = &pw[p][4 * s];
           const auto pb = __builtin_bit_cast(typename VM::v8, make_uint4(pp[0], pp[1], pp[2], pp[3]));
 #pragma unroll
           for (int b = 0; b < DBLK; ++b) {
-            const i16x8_t va = __builtin_shufflevector(lo[b], hi[b], 0, 1, 2, 3, 4, 5, 6, 7);
+            const i16x8_t va = __builtin_shufflevector(vlo[s][b], vhi[s][b], 0, 1, 2, 3, 4, 5, 6, 7);
             o[b] = VM::run(__builtin_bit_cast(typename VM::v8, va), pb, o[b]);
           }
         }
@@ -711,7 +719,7 @@ void attn_tile_kernel(TileArgs a) {
 
   // The piece's tiles [t0, t1) again, key by key: a lane's row against every
   // key of this wavefront that it sees, in the same dims.
-  auto careful = [&](const Unit& u, int t0, int t1) {
+  auto careful = [&](int t0, int t1) {
     m_run = kNegBig;
     l_run = 0.0f;
 #pragma unroll
@@ -722,16 +730,16 @@ void attn_tile_kernel(TileArgs a) {
 #pragma unroll 1
     for (int i = t0 * KPW; i < t1 * KPW; ++i) {
       const int key = i / KPW * KT + kg * KPW + i % KPW;
-      if (key >= u.kend) continue;
+      if (key >= U.kend) continue;
       bool sees = key <= lim;
-      if (TREE && key >= u.committed) {
-        const int tt = key - u.committed;
+      if (TREE && key >= U.committed) {
+        const int tt = key - U.committed;
         sees = sees && (tt >> 6) < a.b.mask_words &&
                (a.b.mask[(int64_t)qrow * a.b.mask_words + (tt >> 6)] >> (tt & 63)) & 1;
       }
       if (!sees) continue;
-      const int64_t phys = physical_block(a.b, a.c.num_blocks, a.seq_begin + u.seq, key / kBs);
-      const int64_t at = phys * a.c.blk + (key % kBs) * a.c.tok + u.kvh * a.c.head;
+      const int64_t phys = physical_block(a.b, a.c.num_blocks, a.seq_begin + U.seq, key / kBs);
+      const int64_t at = phys * a.c.blk + (key % kBs) * a.c.tok + U.kvh * a.c.head;
       const char* kp = (const char*)a.c.kv[0] + at * E::kBytes;
       float x = 0.0f;
 #pragma unroll 1
@@ -744,7 +752,7 @@ void attn_tile_kernel(TileArgs a) {
       x *= a.r.scale_log2;
       float vs = 1.0f;
       if constexpr (kCodes) {
-        const int64_t so = phys * a.c.sblk + (key % kBs) * a.c.stok + u.kvh * a.c.shead;
+        const int64_t so = phys * a.c.sblk + (key % kBs) * a.c.stok + U.kvh * a.c.shead;
         x *= a.c.scale[0][so];
         vs = a.c.scale[1][so];
       }
@@ -772,7 +780,7 @@ void attn_tile_kernel(TileArgs a) {
   };
 
   // Four dims of a row: to the output, or to the piece's slot.
-  auto put = [&](const Unit& u, int slot, int idx, int d, float x0, float x1, float x2, float x3) {
+  auto put = [&](int slot, int idx, int d, float x0, float x1, float x2, float x3) {
     if (slot < 0) {
       T* op = (T*)a.r.out + (int64_t)qrow * a.r.out_stride + (int64_t)qhead * D + d;
       if constexpr (std::is_same<T, float>::value)
@@ -784,17 +792,17 @@ void attn_tile_kernel(TileArgs a) {
           make_float4(x0, x1, x2, x3);
     }
   };
-  auto finish = [&](const Unit& u, int t0, int t1) {
-    float all = l_run, unit = P::kLog ? pow2(u.unit2) : 1.0f;
+  auto finish = [&](int t0, int t1) {
+    float all = l_run, unit = P::kLog ? pow2(U.unit2) : 1.0f;
 #pragma unroll
     for (int b = 0; b < DBLK; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) all += o[b][i];
     if (__ballot(!(fabsf(all) < __builtin_inff()))) {
-      careful(u, t0, t1);
+      careful(t0, t1);
       unit = 1.0f;
     }
-    const bool whole = t0 == 0 && t1 == u.ntiles;
+    const bool whole = t0 == 0 && t1 == U.ntiles;
     const int slot = whole ? -1 : 2 * w + (t0 == 0 ? 1 : 0);
     const int idx = 32 * rg + lr;                  // the row's place in the unit
     l_run = xor32_sum(l_run);
@@ -808,7 +816,7 @@ void attn_tile_kernel(TileArgs a) {
       for (int b = 0; b < DBLK; ++b)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
-          put(u, slot, idx, 32 * b + 8 * q4 + 4 * h, o[b][4 * q4] * inv, o[b][4 * q4 + 1] * inv,
+          put(slot, idx, 32 * b + 8 * q4 + 4 * h, o[b][4 * q4] * inv, o[b][4 * q4 + 1] * inv,
               o[b][4 * q4 + 2] * inv, o[b][4 * q4 + 3] * inv);
     } else {
       constexpr int GRP = DBLK * 4 / KW;           // groups of four dims each wavefront ends with
@@ -850,7 +858,7 @@ void attn_tile_kernel(TileArgs a) {
           s.z = fmaf(v.z, ml[k].x, s.z); s.w = fmaf(v.w, ml[k].x, s.w);
         }
         if (live)
-          put(u, slot, idx, 32 * (grp >> 2) + 8 * (grp & 3) + 4 * h, s.x * inv, s.y * inv,
+          put(slot, idx, 32 * (grp >> 2) + 8 * (grp & 3) + 4 * h, s.x * inv, s.y * inv,
               s.z * inv, s.w * inv);
       }
       team_barrier();                              // the next tile may be written
@@ -858,80 +866,41 @@ void attn_tile_kernel(TileArgs a) {
   };
 
   // -- the range ---------------------------------------------------------------
-  // The tile after (u, tile) at place p of the list: true if there is one;
-  // `inside`: it belongs to the same unit.
-  auto advance = [&](Unit& u, int& tile, int& p, bool& inside) {
-    inside = tile + 1 < u.ntiles && (direct || p + 1 < r1);
-    if (inside) {
-      ++tile;
-      p += direct ? 0 : 1;
-      return true;
-    }
-    if (p + 1 >= r1) return false;
-    ++p;
-    u = next_unit<TREE, RW>(a, u, G);
-    make_uniform(u);
-    tile = 0;
-    return true;
-  };
-  int first = t, p = r0;
-  bool fresh = true;
-  load_tile(U, t, true);
-  if constexpr (NST == 2) {
-    // one tile computed, the next in registers on its way to the other stage,
-    // the one after that being loaded: one barrier per tile
-    Unit N = U;
-    int nt = t, st = 0;
-    bool inside = false;
-    write_tile(U, t, 0);
-    bool more = advance(N, nt, p, inside);
-    if (more) load_tile(N, nt, !inside);
-    team_barrier();
-    while (true) {
-      Unit M = N;
-      int mt = nt;
-      bool then = false, minside = false;
-      if (fresh) start(U);
-      if (more) {
-        write_tile(N, nt, st ^ 1);
-        then = advance(M, mt, p, minside);
-        if (then) load_tile(M, mt, !minside);
-      }
-      compute(U, t, st);
-      fresh = !(more && inside);
-      if (fresh) {
-        finish(U, first, t + 1);
-        first = 0;
-      }
-      if (!more) break;
+  for (int p = r0;;) {
+    const int t1 = direct ? U.ntiles : min(U.ntiles, t + (r1 - p));
+    set_piece(t);
+    load_tile(t);
+    start();
+    if constexpr (NST == 2) {
+      // one tile computed, the next in registers on its way to the other stage,
+      // the one after that being loaded: one barrier per tile
+      write_tile(t, 0);
+      if (t + 1 < t1) load_tile(t + 1);
       team_barrier();
-      U = N; t = nt;
-      N = M; nt = mt;
-      more = then; inside = minside;
-      st ^= 1;
-    }
-  } else {
-    while (true) {
-      if constexpr (RW > 1) team_barrier();        // the last tile has been read
-      write_tile(U, t, 0);
-      if (fresh) start(U);
-      Unit N = U;
-      int nt = t;
-      bool inside = false;
-      const bool more = advance(N, nt, p, inside);
-      if (more) load_tile(N, nt, !inside);
-      if constexpr (RW > 1) team_barrier();
-      else wait_lds();
-      compute(U, t, 0);
-      fresh = !(more && inside);
-      if (fresh) {
-        finish(U, first, t + 1);
-        first = 0;
+      for (int i = t, st = 0; i < t1; ++i, st ^= 1) {
+        if (i + 1 < t1) {
+          write_tile(i + 1, st ^ 1);
+          if (i + 2 < t1) load_tile(i + 2);
+        }
+        compute(i, st);
+        team_barrier();
       }
-      if (!more) break;
-      U = N;
-      t = nt;
+    } else {
+      for (int i = t; i < t1; ++i) {
+        if constexpr (RW > 1) team_barrier();      // the last tile has been read
+        write_tile(i, 0);
+        if (i + 1 < t1) load_tile(i + 1);
+        if constexpr (RW > 1) team_barrier();
+        else wait_lds();
+        compute(i, 0);
+      }
     }
+    finish(t, t1);
+    p += t1 - t;
+    if (direct || p >= r1) break;
+    U = next_unit<TREE, RW>(a, U, G);
+    make_uniform(U);
+    t = 0;
   }
 }
 
