@@ -210,12 +210,12 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
     // contexts of a few tiles are not split where all units run at once (a
     // join takes as long as two tiles or three); where there are half as many
     // units again as run at once, the kernel looks whether they need to be
-    p.direct = tiles <= (one_round ? 4 : 2) ? 2 : 2 * units >= 3 * p.ranges ? 1 : 0;
+    p.direct = one_round && tiles <= 4 ? 3 : tiles <= 2 ? 2 : 2 * units >= 3 * p.ranges ? 1 : 0;
     if (p.direct) p.grid = (int)std::max<int64_t>(all, p.direct == 1 ? p.ranges : 0);
   }
   p.slot_heads = 1;
   p.slot_rows = (int)std::min<int64_t>(rows, r);
-  if (codes && dtype != LV_F32 && rows <= 8 && !(p.direct == 2 && one_round)) {
+  if (codes && dtype != LV_F32 && rows <= 8 && p.direct != 3) {
     p.rw = 0;
     p.direct = 0;
     p.slot_heads = std::min(num_kv_heads, 8);
@@ -223,7 +223,7 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
     const int64_t list = (int64_t)n_seqs * (num_kv_heads / p.slot_heads) * ((max_blocks + 1) / 2);
     p.grid = p.ranges = (int)std::min<int64_t>(list, cus * (8 / p.slot_heads));
   }
-  if (p.direct != 2) {
+  if (p.direct < 2) {
     const size_t slots = (size_t)2 * p.ranges * p.slot_heads * p.slot_rows;
     p.head_bytes = align256((size_t)p.ranges * 2 * 16);
     p.ml_bytes = align256(slots * 8);

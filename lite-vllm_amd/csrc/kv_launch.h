@@ -38,7 +38,7 @@ int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
   const TileArgs t = tile_args(a, p, ws);
   const size_t lds = F::lds(D) + (size_t)(p.n_seqs + 1) * 4;
   attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, kTileThreads, lds, a.stream>>>(t);
-  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct == 2 || p.ranges < 2)
+  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct >= 2 || p.ranges < 2)
     return rc;
   return launch_join<T, D>(a, p, t);
 }

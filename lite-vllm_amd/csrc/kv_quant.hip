@@ -75,13 +75,13 @@ __global__ __launch_bounds__(kQuantThreads) void kv_scatter_quant_kernel(
   const int hs = (int)(row - t * (2 * num_kv_heads));
   const int kv = hs >= num_kv_heads, head = hs - kv * num_kv_heads;
   const int64_t slot = slots[t];
+  float x[8];       // (loaded beside the slot, not after it)
+  load8<T, VEC>((kv ? value + t * value_stride : key + t * key_stride) + (int64_t)head * D + i, x);
   if (slot < 0) return;                      // padding
   if (slot >= c.num_slots) {                 // outside the cache: not written, reported
     if (hs == 0 && i == 0) report_device_error(LV_DEVERR_SLOT);
     return;
   }
-  float x[8];
-  load8<T, VEC>((kv ? value + t * value_stride : key + t * key_stride) + (int64_t)head * D + i, x);
   const float scale = row_scale<C, W, 8>(x);
   const int64_t blk = slot / c.block_size;
   const int off = (int)(slot - blk * c.block_size);
@@ -142,17 +142,17 @@ __global__ __launch_bounds__(kQuantThreads) void qk_norm_rope_cache_quant_kernel
   load8<T, VEC>(src, x);
   load8<T, VEC>(src + HALF, x + 8);
   const bool is_q = hs < num_heads, is_v = hs >= num_heads + num_kv_heads;
+  const T* nw = is_q ? q_norm_w : is_v ? nullptr : k_norm_w;
+  float w[16];
+  if (nw) {
+    load8<T, VEC>(nw + i, w);
+    load8<T, VEC>(nw + i + HALF, w + 8);
+  }
   if (!is_q) {       // padding, and slots outside the cache (reported): nothing is written
     if (slot >= c.num_slots && hs == num_heads && i == 0) report_device_error(LV_DEVERR_SLOT);
     if (slot < 0 || slot >= c.num_slots) return;
   }
   if (!is_v) {
-    const T* nw = is_q ? q_norm_w : k_norm_w;
-    float w[16];
-    if (nw) {
-      load8<T, VEC>(nw + i, w);
-      load8<T, VEC>(nw + i + HALF, w + 8);
-    }
     // a position without a cos / sin row makes the output NaN
     const bool pos_ok = pos >= 0 && pos < max_position;
     const int64_t prow = (pos_ok ? pos : 0) * HALF + i;

@@ -58,7 +58,8 @@ struct TileArgs {
   Batch b; KvView c; Rows r;
   int seq_begin, n_seqs, max_q;
   int ranges;               // ranges of the list
-  int direct;               // a workgroup per unit: 2 always, 1 if no unit is long
+  int direct;               // a workgroup per unit: 1 if no unit is long, 2 always, 3 always
+                            // and in no order (all run at once)
   int nq;                   // row tiles of a unit's sequence, at most
   int slot_heads, slot_rows;   // kv heads of a workspace slot, rows of each
   int4* head;               // [ranges][2]: the unit that crosses a range's start
@@ -155,7 +156,7 @@ __device__ int scan_tiles(const TileArgs& a, int g, int* off, int* part) {
 // context (ties by index) where they are few enough to rank, r otherwise.
 constexpr int kRankMax = kTileThreads;
 __device__ __forceinline__ int ranked_sequence(const TileArgs& a, int r, int* ctx, int* pick) {
-  if (a.n_seqs > kRankMax) return r;
+  if (a.n_seqs > kRankMax || a.direct == 3) return r;
   const int t = threadIdx.x;
   const int mine = t < a.n_seqs ? tile_sequence(a, t).ctx : -1;
   ctx[t] = mine;
@@ -347,7 +348,7 @@ void attn_tile_kernel(TileArgs a) {
   const int lr = lane & 31, h = lane >> 5;
 
   int r0 = 0, r1 = 1, w = 0, t = 0, per = 1;
-  bool direct = a.direct == 2;
+  bool direct = a.direct >= 2;
   if (!direct) {
     const int longest = uniform(scan_tiles<TREE, RW>(a, G, s_off, s_part));
     const int total = uniform(s_off[a.n_seqs]);
@@ -414,27 +415,6 @@ void attn_tile_kernel(TileArgs a) {
     }
     id_first = first;
   };
-  auto set_piece = [&](int first) {
-    kbase = (const char*)a.c.kv[0] + U.kvh * a.c.head * E::kBytes;
-    vbase = (const char*)a.c.kv[1] + U.kvh * a.c.head * E::kBytes;
-    load_ids(first);
-    if constexpr (kCodes) {
-      // lanes 0 .. 16 BPW - 1 the K scales, the next as many the V scales
-      const bool of_v = (lane / (16 * BPW)) & 1;
-      sbase = (of_v ? a.c.scale[1] : a.c.scale[0]) + (lane & 15) * a.c.stok + U.kvh * a.c.shead;
-    }
-    if constexpr (P::kLog) {     // the unit of the V scales: the largest of the first 64
-      float v = 0.0f;
-      const int key = first * KT + lane;
-      if (key < U.kend) {
-        const int64_t phys = physical_block(a.b, a.c.num_blocks, a.seq_begin + U.seq, key / kBs);
-        v = a.c.scale[1][phys * a.c.sblk + (key % kBs) * a.c.stok + U.kvh * a.c.shead];
-      }
-      v = group_max<64>(v > 0.0f && v < __builtin_inff() ? v : 0.0f);
-      const int e = uniform((int)(__float_as_uint(v) >> 23));      // 0: no scale
-      U.unit2 = e > 0 ? min(max(e - 127, -100), 100) : 0;
-    }
-  };
   auto load_tile = [&](int tile) {
     if (tile - id_first >= 64) load_ids(tile);
     int phys[BPW];     // (read by all lanes: a readlane under a branch sees stale copies)
@@ -452,6 +432,31 @@ void attn_tile_kernel(TileArgs a) {
     if constexpr (kCodes) {
       const int block = lane & 16 ? phys[BPW - 1] : phys[0];
       sraw = sbase[block * a.c.sblk];
+    }
+  };
+  // Loads the piece's first tile; what they wait for one after the other (block
+  // table, then rows) is in flight with the look at the V scales.
+  auto set_piece = [&](int first) {
+    kbase = (const char*)a.c.kv[0] + U.kvh * a.c.head * E::kBytes;
+    vbase = (const char*)a.c.kv[1] + U.kvh * a.c.head * E::kBytes;
+    load_ids(first);
+    const int key = first * KT + lane;
+    int block = 0;
+    if (P::kLog && key < U.kend)
+      block = physical_block(a.b, a.c.num_blocks, a.seq_begin + U.seq, key / kBs);
+    if constexpr (kCodes) {
+      // lanes 0 .. 16 BPW - 1 the K scales, the next as many the V scales
+      const bool of_v = (lane / (16 * BPW)) & 1;
+      sbase = (of_v ? a.c.scale[1] : a.c.scale[0]) + (lane & 15) * a.c.stok + U.kvh * a.c.shead;
+    }
+    load_tile(first);
+    if constexpr (P::kLog) {     // the unit of the V scales: the largest of the first 64
+      float v = 0.0f;
+      if (key < U.kend)
+        v = a.c.scale[1][block * a.c.sblk + (key % kBs) * a.c.stok + U.kvh * a.c.shead];
+      v = group_max<64>(v > 0.0f && v < __builtin_inff() ? v : 0.0f);
+      const int e = uniform((int)(__float_as_uint(v) >> 23));      // 0: no scale
+      U.unit2 = e > 0 ? min(max(e - 127, -100), 100) : 0;
     }
   };
   auto write_tile = [&](int tile, int st) {
@@ -869,7 +874,6 @@ void attn_tile_kernel(TileArgs a) {
   for (int p = r0;;) {
     const int t1 = direct ? U.ntiles : min(U.ntiles, t + (r1 - p));
     set_piece(t);
-    load_tile(t);
     start();
     if constexpr (NST == 2) {
       // one tile computed, the next in registers on its way to the other stage,
