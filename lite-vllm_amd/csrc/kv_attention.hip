@@ -15,114 +15,6 @@
 
 namespace lv {
 
-// One workgroup of 4 wavefronts per (query row, head).  A lane takes one key
-// of 64 for the scores (its whole row, against the query in LDS), then one or
-// two dims for the output (every key's weight broadcast by readlane), so no
-// row of the cache is ever spread and summed over lanes.  Right for every
-// type and mask, and the form that the others are held to: it reads the cache
-// once for every query row and head.
-template <typename T, typename C, int D, bool TREE>
-__global__ __launch_bounds__(256) void attn_row_kernel(Batch b, KvView c, Rows r) {
-  using E = cached<C>;
-  constexpr int P = E::kPer16B, DPL = D / 64;
-  __shared__ float s_q[D];
-  __shared__ float s_o[4][D];
-  __shared__ float s_ml[4][2];
-  const int row = blockIdx.x, head = blockIdx.y;
-  int seq = row;
-  if (b.cu) {
-    int lo = 0, hi = b.num_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (b.cu[mid] <= row) lo = mid; else hi = mid - 1;
-    }
-    seq = lo;
-  }
-  const Seq s = sequence(b, seq);
-  const int j = row - s.q0;
-  if (j < 0 || j >= s.n) return;
-  const int kvh = head / (r.num_heads / r.num_kv_heads);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const T* qp = (const T*)r.q + (int64_t)row * r.q_stride + (int64_t)head * D;
-  for (int d = threadIdx.x; d < D; d += 256) s_q[d] = elem<T>::load(qp + d) * r.scale_log2;
-  __syncthreads();
-  const char* kb = (const char*)c.kv[0] + (int64_t)kvh * c.head * E::kBytes;
-  const char* vb = (const char*)c.kv[1] + (int64_t)kvh * c.head * E::kBytes;
-  const int committed = s.ctx - s.n;
-  const int end = TREE ? s.ctx : min(s.ctx, committed + j + 1);
-  float m = kNegBig, l = 0.0f, o[DPL] = {};
-  for (int k0 = wave * 64; k0 < end; k0 += 256) {
-    const int key = k0 + lane;
-    bool sees = key < end;
-    if (TREE && sees && key >= committed) {
-      const int t = key - committed;
-      sees = (b.mask[(int64_t)row * b.mask_words + (t >> 6)] >> (t & 63)) & 1;
-    }
-    const int kc = min(key, end - 1);
-    const int64_t phys = physical_block(b, c.num_blocks, seq, kc / kBs);
-    const int off = kc % kBs;
-    const char* kp = kb + (phys * c.blk + off * c.tok) * E::kBytes;
-    float x = 0.0f;
-    for (int d = 0; d < D; d += P) {
-      float kf[P];
-      E::unpack(load16(kp + d * E::kBytes), kf);
-#pragma unroll
-      for (int i = 0; i < P; ++i) x = fmaf(s_q[d + i], kf[i], x);
-    }
-    float vs = 1.0f;
-    if constexpr (E::kCodes) {
-      const int64_t at = phys * c.sblk + off * c.stok + kvh * c.shead;
-      x *= c.scale[0][at];
-      vs = c.scale[1][at];
-    }
-    const float mx = fmaxf(m, group_max<64>(sees ? x : kNegBig));
-    const float alpha = fast_exp2(m - mx);
-    m = mx;
-    const float p = sees ? fast_exp2(x - m) : 0.0f;
-    l = l * alpha + p;
-    const float w = p * vs;
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) o[i] *= alpha;
-    uint64_t seen = __ballot(sees);
-    const int64_t vat = (phys * c.blk + off * c.tok) * E::kBytes;
-    while (seen) {       // (a key that is not seen is not read: it may hold anything)
-      const int k = __builtin_ctzll(seen);
-      seen &= seen - 1;
-      const float wk = __shfl(w, k);
-      const char* vp = vb + __shfl(vat, k);
-#pragma unroll
-      for (int i = 0; i < DPL; ++i) {
-        const int d = lane + 64 * i;
-        float v;
-        if constexpr (E::kCodes) {
-          float four[4];
-          code<C>::unpack4(*(const uint8_t*)(vp + d), four);
-          v = four[0];
-        } else {
-          v = elem<C>::load((const C*)vp + d);
-        }
-        o[i] = fmaf(wk, v, o[i]);
-      }
-    }
-  }
-  l = group_sum<64>(l);
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) s_o[wave][lane + 64 * i] = o[i];
-  if (lane == 0) { s_ml[wave][0] = m; s_ml[wave][1] = l; }
-  __syncthreads();
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float mx = kNegBig, sum = 0.0f, acc = 0.0f;
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_ml[w][0]);
-    for (int w = 0; w < 4; ++w) {
-      const float f = fast_exp2(s_ml[w][0] - mx);
-      sum = fmaf(s_ml[w][1], f, sum);
-      acc = fmaf(s_o[w][d], f, acc);
-    }
-    elem<T>::store((T*)r.out + (int64_t)row * r.out_stride + (int64_t)head * D + d,
-                   sum != 0.0f ? acc / sum : 0.0f);
-  }
-}
-
 // Ancestor bits: thread per drafted token walks up its parents, whose indices
 // fall, so that every walk ends.
 __global__ __launch_bounds__(256) void tree_mask_kernel(const int32_t* __restrict__ parents,
@@ -158,18 +50,6 @@ LV_ERROR_WORD_READER(read_errors_tree)
 // Host side.
 // ---------------------------------------------------------------------------
 namespace {
-
-template <typename T, typename C, int D>
-int launch_rows(const Call& a) {
-  const dim3 grid((unsigned)a.b.num_tokens, (unsigned)a.r.num_heads);
-  if (a.tree) attn_row_kernel<T, C, D, true><<<grid, 256, 0, a.stream>>>(a.b, a.c, a.r);
-  else attn_row_kernel<T, C, D, false><<<grid, 256, 0, a.stream>>>(a.b, a.c, a.r);
-  return check_launch("attn_row_kernel");
-}
-
-int launch_rows(const Call& a) {      // an fp32 cache
-  return a.d == 64 ? launch_rows<float, float, 64>(a) : launch_rows<float, float, 128>(a);
-}
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -259,17 +139,20 @@ int launch_part(const Call& a, const TilePlan& p, char* ws) {
 
 int launch(const Call& a, int num_decodes, int max_query_len, void* ws) {
   const int h = a.r.num_heads, hkv = a.r.num_kv_heads, mb = a.b.max_blocks;
-  if (a.code < 0 && a.dtype == LV_F32) return launch_rows(a);
   // (the narrow kernel's offsets within a block are 32 bits wide)
   const bool codes = a.code >= 0 && a.c.tok <= (1 << 26);
   if (num_decodes > 0) {
     const TilePlan p = plan_tiles(0, num_decodes, 1, h, hkv, a.d, mb, a.dtype, codes);
     if (const int rc = launch_part(a, p, (char*)ws); rc != LV_OK) return rc;
   }
-  if (num_decodes == a.b.num_seqs) return LV_OK;
-  return launch_part(a, plan_tiles(num_decodes, a.b.num_seqs - num_decodes, max_query_len, h, hkv,
-                                   a.d, mb, a.dtype, codes),
-                     (char*)ws);
+  // (fp32 operands leave the LDS of a CU room for so many sequences' offsets)
+  const int most = a.code < 0 && a.dtype == LV_F32 ? 4096 : a.b.num_seqs;
+  for (int i = num_decodes; i < a.b.num_seqs; i += most) {
+    const TilePlan p = plan_tiles(i, std::min(most, a.b.num_seqs - i), max_query_len, h, hkv, a.d,
+                                  mb, a.dtype, codes);
+    if (const int rc = launch_part(a, p, (char*)ws); rc != LV_OK) return rc;
+  }
+  return LV_OK;
 }
 
 // The checks common to the attention entries; fills `a` but for the cache.

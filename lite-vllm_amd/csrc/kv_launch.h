@@ -36,7 +36,7 @@ template <typename T, typename C, int D, int RW, bool TREE>
 int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
   using F = TileCfg<RW>;
   const TileArgs t = tile_args(a, p, ws);
-  const size_t lds = F::lds(D) + (size_t)(p.n_seqs + 1) * 4;
+  const size_t lds = F::lds(D, Operands<T, C>::kWide ? 4 : 2) + (size_t)(p.n_seqs + 1) * 4;
   attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, kTileThreads, lds, a.stream>>>(t);
   if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct >= 2 || p.ranges < 2)
     return rc;
@@ -81,9 +81,7 @@ int launch_tiles(const Call& a, const TilePlan& p, char* ws) {
   if (a.code == LV_E4M3)
     return a.d == 64 ? launch_tiles_d<T, e4m3_code, 64>(a, p, ws)
                      : launch_tiles_d<T, e4m3_code, 128>(a, p, ws);
-  if constexpr (!std::is_same<T, float>::value)
-    return a.d == 64 ? launch_tiles_d<T, T, 64>(a, p, ws) : launch_tiles_d<T, T, 128>(a, p, ws);
-  return LV_ERR_UNSUPPORTED;
+  return a.d == 64 ? launch_tiles_d<T, T, 64>(a, p, ws) : launch_tiles_d<T, T, 128>(a, p, ws);
 }
 
 }  // namespace lv

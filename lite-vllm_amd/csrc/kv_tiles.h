@@ -87,8 +87,8 @@ template <int RW> struct TileCfg {
   static constexpr int BPW = KT / 64;             // 16-token blocks a wavefront stages
   static constexpr int KPW = KT / KW;             // keys a wavefront computes
   static constexpr int NST = RW == 4 ? 2 : 1;     // LDS stages
-  static constexpr size_t lds(int d) {            // without the list's offsets
-    return (size_t)NST * (KT * d * 4 + KT * 12) + 128 * 8;
+  static constexpr size_t lds(int d, int bytes) { // operands of so many bytes; without the
+    return (size_t)NST * (KT * d * 2 * bytes + KT * 12) + 128 * 8;      // list's offsets
   }
 };
 
@@ -302,6 +302,7 @@ template <typename T, typename C> struct Operands {
                                       K>::type;
   static constexpr int QP = kF32 ? 3 : 1;
   static constexpr int PP = kF32 ? 3 : std::is_same<V, f16>::value ? 1 : 2;
+  static constexpr bool kWide = std::is_same<C, float>::value;   // fp32 operands
   // A row's reference is set kLift (in log2 units) under the score that sets it
   // and again when a score passes it by kTop: fp16 weights then lie high enough
   // that the fixed step of the smallest ones, 2^-24, weighs nothing.
@@ -327,12 +328,14 @@ void attn_tile_kernel(TileArgs a) {
   constexpr int CPR = D / E::kPer16B;             // 16-byte chunks of a cached row
   constexpr int RPL = 64 / CPR;                   // rows of a wavefront-wide load
   constexpr int LPB = kBs / RPL;                  // loads of a block's K or V
-  constexpr int OPC = E::kPer16B / 8;             // operand chunks of a cached chunk
+  constexpr int OPC = E::kPer16B < 8 ? 1 : E::kPer16B / 8;             // operand chunks of a cached chunk
+  constexpr bool kWide = P::kWide;
   static_assert(16 % RPL == 0, "whole loads per block");
   // K and V tile, then the scales of its keys; the merge of a piece's parts
   // reuses the tiles (4 wavefronts x 32 rows x D floats at most)
   extern __shared__ __align__(16) unsigned char s_dyn[];
-  constexpr int NST = F::NST, TILE = KT * D;       // (elements of K or V)
+  // (of K or V, in 16-bit places)
+  constexpr int NST = F::NST, TILE = KT * D * (kWide ? 2 : 1);
   uint16_t* const s_kv = reinterpret_cast<uint16_t*>(s_dyn);       // [NST][K, V][TILE]
   // [NST][KT] each: K's scales; V's scales, or their logarithms and inverses
   float* const s_sc = reinterpret_cast<float*>(s_kv + NST * 2 * TILE);
@@ -470,18 +473,23 @@ void attn_tile_kernel(TileArgs a) {
       for (int i = 0; i < LPB; ++i) {
         const int row = 16 * (wave * BPW + j) + RPL * i + lrow;    // of the tile
         if (tail && tile * KT + row >= U.kend) vraw[j][i] = make_uint4(0, 0, 0, 0);
-        uint4 ko[OPC], vo[OPC];
-        if constexpr (kCodes) {
-          codes_to_operands<typename P::K, C>(kraw[j][i], ko);
-          codes_to_operands<typename P::V, C>(vraw[j][i], vo);
+        if constexpr (kWide) {
+          store16(Ks + 2 * row * D + 8 * (lchunk ^ (row & 15)), kraw[j][i]);
+          store16(Vs + 2 * row * D + 8 * (lchunk ^ (2 * (row & 4))), vraw[j][i]);
         } else {
-          ko[0] = kraw[j][i];
-          vo[0] = vraw[j][i];
-        }
+          uint4 ko[OPC], vo[OPC];
+          if constexpr (kCodes) {
+            codes_to_operands<typename P::K, C>(kraw[j][i], ko);
+            codes_to_operands<typename P::V, C>(vraw[j][i], vo);
+          } else {
+            ko[0] = kraw[j][i];
+            vo[0] = vraw[j][i];
+          }
 #pragma unroll
-        for (int c = 0; c < OPC; ++c) {
-          store16(Ks + L::at(row, lchunk * OPC + c), ko[c]);
-          store16(Vs + L::at(row, lchunk * OPC + c), vo[c]);
+          for (int c = 0; c < OPC; ++c) {
+            store16(Ks + L::at(row, lchunk * OPC + c), ko[c]);
+            store16(Vs + L::at(row, lchunk * OPC + c), vo[c]);
+          }
         }
       }
     if constexpr (kCodes) {
@@ -506,7 +514,8 @@ void attn_tile_kernel(TileArgs a) {
 
   // -- a piece's state -------------------------------------------------------
   using qv8 = typename KM::v8;
-  qv8 qf[P::QP][QSTEPS];
+  qv8 qf[kWide ? 1 : P::QP][kWide ? 1 : QSTEPS];
+  float4 qw[kWide ? D / 8 : 1];              // fp32 operands: dims 8 i + 4 h ...
   f32x16_t o[DBLK];
   float m_run = kNegBig, l_run = 0.0f;
   int qrow = 0, qhead = 0, lim = 0;          // this lane's row, head and last key
@@ -520,7 +529,14 @@ void attn_tile_kernel(TileArgs a) {
     qhead = U.kvh * G + use % G;
     lim = TREE ? U.kend - 1 : min(U.committed + use / G, U.kend - 1);
     const T* qp = (const T*)a.r.q + (int64_t)qrow * a.r.q_stride + (int64_t)qhead * D + 8 * h;
-    if constexpr (P::QP == 1) {
+    if constexpr (kWide) {
+      uint4 raw[D / 8];
+#pragma unroll
+      for (int s = 0; s < D / 8; ++s) raw[s] = load16(qp - 4 * h + 8 * s);
+      settle(raw);
+#pragma unroll
+      for (int s = 0; s < D / 8; ++s) qw[s] = __builtin_bit_cast(float4, raw[s]);
+    } else if constexpr (P::QP == 1) {
       uint4 raw[QSTEPS];
 #pragma unroll
       for (int s = 0; s < QSTEPS; ++s) raw[s] = load16(qp + 16 * s);
@@ -575,14 +591,38 @@ void attn_tile_kernel(TileArgs a) {
 
   auto compute = [&](int tile, int st) {
     const int k0 = tile * KT + kg * KPW;           // this wavefront's first key
-    const uint32_t kt = (uint32_t)(2 * (st * 2 * TILE + kg * KPW * D)), vt = kt + 2 * TILE;
+    const uint32_t kt = (uint32_t)(2 * st * 2 * TILE + (kWide ? 4 : 2) * kg * KPW * D);
+    const uint32_t vt = kt + 2 * TILE;
     const float* const s_ks = s_sc + st * 3 * KT + kg * KPW;
     const float* const s_vs = s_ks + KT;
     // Four K operands in flight: read j + 4 goes out when product j has taken
     // its buffer (left to itself, the compiler waits out each read in turn).
     f32x16_t sv[KB];
     __builtin_amdgcn_s_setprio(1);
-    {
+    if constexpr (kWide) {
+      // a step of two dims: d from half h = 0, d + 4 from h = 1
+      constexpr int NJ = KB * (D / 8);
+      auto kread = [&](int j) __attribute__((always_inline)) {
+        const int chunk = 2 * (j % (D / 8)) + h;
+        return *reinterpret_cast<const float4*>(
+            s_dyn + kt + 4 * (32 * (j / (D / 8)) + lr) * D + 16 * (chunk ^ (lr & 15)));
+      };
+      float4 ka[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) ka[j] = kread(j);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int kb = j / (D / 8), s = j % (D / 8);
+        if (s == 0) sv[kb] = f32x16_t{};
+        sv[kb] = mfma32_f32(ka[j & 1].x, qw[s].x, sv[kb]);
+        sv[kb] = mfma32_f32(ka[j & 1].y, qw[s].y, sv[kb]);
+        sv[kb] = mfma32_f32(ka[j & 1].z, qw[s].z, sv[kb]);
+        sv[kb] = mfma32_f32(ka[j & 1].w, qw[s].w, sv[kb]);
+        if (j + 2 < NJ) ka[j & 1] = kread(j + 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
       constexpr int NJ = KB * QSTEPS;
       auto kread = [&](int j) __attribute__((always_inline)) {
         return *reinterpret_cast<const uint4*>(
@@ -692,6 +732,21 @@ void attn_tile_kernel(TileArgs a) {
             sv[kb][4 * q4 + 2] *= vs.z; sv[kb][4 * q4 + 3] *= vs.w;
           }
         }
+      }
+      if constexpr (kWide) {
+        // a step of two keys: 8 q4 + e from half h = 0, 4 more from h = 1, as
+        // the scores lie
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = 32 * kb + 8 * (i >> 2) + (i & 3) + 4 * h;
+#pragma unroll
+          for (int b = 0; b < DBLK; ++b) {
+            const float v = *reinterpret_cast<const float*>(
+                s_dyn + vt + 4 * key * D + 16 * ((8 * b + (lr >> 2)) ^ (8 * h)) + 4 * (lr & 3));
+            o[b] = mfma32_f32(v, sv[kb][i], o[b]);
+          }
+        }
+        continue;
       }
       uint32_t pw[P::PP][8];
 #pragma unroll

@@ -40,6 +40,11 @@ template <> struct Mfma32<f16> {
   }
 };
 
+// 32 x 32 x 2 of fp32 values: A[i][k] is lane i + 32 k, B[k][j] lane j + 32 k.
+__device__ __forceinline__ f32x16_t mfma32_f32(float a, float b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
 // 16 x 16 instructions (the matrix-core decode kernel).  Layouts:
 //   A[i][k]: lane i + 16 * (k / E), element k % E    (E = 8: K = 32; E = 4: K = 16)
 //   B[k][j]: lane j + 16 * (k / E), element k % E
