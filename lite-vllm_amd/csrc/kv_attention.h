@@ -32,7 +32,7 @@ struct Rows {
 };
 
 constexpr int kBs = 16;
-constexpr float kNegBig = -1.0e30f;
+constexpr float kNegBig = -3.40282347e38f;     // under every finite score
 
 template <typename C> struct cached {          // 8-bit codes
   static constexpr bool kCodes = true;
@@ -83,7 +83,7 @@ struct Call {
 // most: their kernel, its launch and its workspace.
 struct TilePlan {
   int seq_begin, n_seqs, max_q;
-  int rw;                   // tile kernel: 32-row groups of a unit, 1, 2 or 4; 0: narrow kernel
+  int rw;                   // tile kernel: 32-row groups of a unit, 1, 2, 4 or 8; 0: narrow kernel
   int grid, ranges;         // workgroups; ranges that the list is split into
   int direct, nq;           // (see TileArgs)
   int slot_heads, slot_rows;

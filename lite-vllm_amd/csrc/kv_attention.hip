@@ -76,15 +76,16 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   p.n_seqs = n_seqs;
   p.max_q = max_q;
   const int64_t rows = std::max<int64_t>(1, (int64_t)max_q * (num_heads / num_kv_heads));
-  p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || dtype == LV_F32 ? 4 : 8;
   const int r = 32 * p.rw, kt = p.rw == 4 ? 64 : 128;
   const int64_t units = (int64_t)n_seqs * num_kv_heads * ((rows + r - 1) / r);
   const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_blocks * kBs + kt - 1) / kt);
   const int64_t cus = device_cus();
   p.nq = (int)((rows + r - 1) / r);
-  p.ranges = (int)std::min<int64_t>(units * tiles, cus * (dtype == LV_F32 ? 1 : 2));
+  const int64_t at_once = cus * (dtype == LV_F32 || p.rw == 8 ? 1 : 2);
+  p.ranges = (int)std::min<int64_t>(units * tiles, at_once);
   p.grid = p.ranges;
-  const bool one_round = units <= cus * (dtype == LV_F32 ? 1 : 2);
+  const bool one_round = units <= at_once;
   const int64_t all = ((int64_t)n_seqs * num_kv_heads + kXcds - 1) / kXcds * kXcds * p.nq;
   if (all < (1ll << 31)) {
     // contexts of a few tiles are not split where all units run at once (a
@@ -145,8 +146,8 @@ int launch(const Call& a, int num_decodes, int max_query_len, void* ws) {
     const TilePlan p = plan_tiles(0, num_decodes, 1, h, hkv, a.d, mb, a.dtype, codes);
     if (const int rc = launch_part(a, p, (char*)ws); rc != LV_OK) return rc;
   }
-  // (fp32 operands leave the LDS of a CU room for so many sequences' offsets)
-  const int most = a.code < 0 && a.dtype == LV_F32 ? 4096 : a.b.num_seqs;
+  // (the largest tiles leave the LDS of a CU room for so many sequences' offsets)
+  constexpr int most = 4096;
   for (int i = num_decodes; i < a.b.num_seqs; i += most) {
     const TilePlan p = plan_tiles(i, std::min(most, a.b.num_seqs - i), max_query_len, h, hkv, a.d,
                                   mb, a.dtype, codes);

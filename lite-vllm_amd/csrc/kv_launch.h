@@ -37,7 +37,7 @@ int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
   using F = TileCfg<RW>;
   const TileArgs t = tile_args(a, p, ws);
   const size_t lds = F::lds(D, Operands<T, C>::kWide ? 4 : 2) + (size_t)(p.n_seqs + 1) * 4;
-  attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, kTileThreads, lds, a.stream>>>(t);
+  attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, F::THREADS, lds, a.stream>>>(t);
   if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct >= 2 || p.ranges < 2)
     return rc;
   return launch_join<T, D>(a, p, t);
@@ -63,12 +63,16 @@ int launch_tiles_d(const Call& a, const TilePlan& p, char* ws) {
   if (a.tree) {
     if (p.rw == 1) return launch_tile_kernel<T, C, D, 1, true>(a, p, ws);
     if (p.rw == 2) return launch_tile_kernel<T, C, D, 2, true>(a, p, ws);
-    return launch_tile_kernel<T, C, D, 4, true>(a, p, ws);
+    if (std::is_same<T, float>::value || p.rw == 4)
+      return launch_tile_kernel<T, C, D, 4, true>(a, p, ws);
+    return launch_tile_kernel<T, C, D, std::is_same<T, float>::value ? 4 : 8, true>(a, p, ws);
   }
   if constexpr (cached<C>::kCodes) {
     if (p.rw == 1) return launch_tile_kernel<T, C, D, 1, false>(a, p, ws);
     if (p.rw == 2) return launch_tile_kernel<T, C, D, 2, false>(a, p, ws);
-    return launch_tile_kernel<T, C, D, 4, false>(a, p, ws);
+    if (std::is_same<T, float>::value || p.rw == 4)
+      return launch_tile_kernel<T, C, D, 4, false>(a, p, ws);
+    return launch_tile_kernel<T, C, D, std::is_same<T, float>::value ? 4 : 8, false>(a, p, ws);
   }
   return LV_ERR_UNSUPPORTED;
 }

@@ -52,8 +52,6 @@ namespace lv {
 // are not finite is computed again key by key (careful), where a key that a
 // row does not see is not read.
 // ---------------------------------------------------------------------------
-constexpr int kTileThreads = 256;
-
 struct TileArgs {
   Batch b; KvView c; Rows r;
   int seq_begin, n_seqs, max_q;
@@ -82,11 +80,13 @@ __device__ __forceinline__ void make_uniform(Unit& u) {
 }
 
 template <int RW> struct TileCfg {
-  static constexpr int R = 32 * RW, KW = 4 / RW;
+  static constexpr int WAVES = RW == 8 ? 8 : 4, THREADS = 64 * WAVES;
+  static constexpr int R = 32 * RW, KW = WAVES / RW;
   static constexpr int KT = RW == 4 ? 64 : 128;   // keys per tile
-  static constexpr int BPW = KT / 64;             // 16-token blocks a wavefront stages
+  static constexpr int BPW = KT / (16 * WAVES);   // 16-token blocks a wavefront stages
   static constexpr int KPW = KT / KW;             // keys a wavefront computes
-  static constexpr int NST = RW == 4 ? 2 : 1;     // LDS stages
+  static constexpr int SUB = KPW > 64 ? 2 : 1;    // in so many steps
+  static constexpr int NST = RW >= 4 ? 2 : 1;     // LDS stages
   static constexpr size_t lds(int d, int bytes) { // operands of so many bytes; without the
     return (size_t)NST * (KT * d * 2 * bytes + KT * 12) + 128 * 8;      // list's offsets
   }
@@ -124,7 +124,7 @@ template <bool TREE, int RW>
 __device__ int scan_tiles(const TileArgs& a, int g, int* off, int* part) {
   using F = TileCfg<RW>;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int per = (a.n_seqs + kTileThreads - 1) / kTileThreads;
+  const int per = (a.n_seqs + F::THREADS - 1) / F::THREADS;
   const int lo = min(a.n_seqs, t * per), hi = min(a.n_seqs, lo + per);
   int sum = 0, longest = 0;
   for (int i = lo; i < hi; ++i) {
@@ -141,20 +141,20 @@ __device__ int scan_tiles(const TileArgs& a, int g, int* off, int* part) {
     if (lane >= d) incl += u;
   }
   if (lane == 63) part[wave] = incl;
-  if (lane == 0) part[4 + wave] = longest;
+  if (lane == 0) part[8 + wave] = longest;
   __syncthreads();
   int base = incl - sum;
   for (int w = 0; w < wave; ++w) base += part[w];
   for (int i = lo; i < hi; ++i) off[i] += base;
-  if (t == kTileThreads - 1) off[a.n_seqs] = base + sum;
-  for (int w = 0; w < 4; ++w) longest = max(longest, part[4 + w]);
+  if (t == F::THREADS - 1) off[a.n_seqs] = base + sum;
+  for (int w = 0; w < F::WAVES; ++w) longest = max(longest, part[8 + w]);
   __syncthreads();
   return longest;
 }
 
 // The sequence that direct workgroups of rank r take: the r-th by descending
 // context (ties by index) where they are few enough to rank, r otherwise.
-constexpr int kRankMax = kTileThreads;
+constexpr int kRankMax = 256;
 __device__ __forceinline__ int ranked_sequence(const TileArgs& a, int r, int* ctx, int* pick) {
   if (a.n_seqs > kRankMax || a.direct == 3) return r;
   const int t = threadIdx.x;
@@ -310,11 +310,11 @@ template <typename T, typename C> struct Operands {
   static constexpr float kTop = std::is_same<V, f16>::value ? 15.0f : 8.0f;
 };
 
-// Workgroups per CU: the three parts of fp32 queries need the registers of two.
-template <typename T> constexpr int kTileWgs = std::is_same<T, float>::value ? 1 : 2;
+// Wavefronts per SIMD: the three parts of fp32 queries need the registers of two.
+template <typename T> constexpr int kTileWaves = std::is_same<T, float>::value ? 1 : 2;
 
 template <typename T, typename C, int D, int RW, bool TREE>
-__global__ __launch_bounds__(kTileThreads, kTileWgs<T>)
+__global__ __launch_bounds__(TileCfg<RW>::THREADS, kTileWaves<T>)
 void attn_tile_kernel(TileArgs a) {
   using F = TileCfg<RW>;
   using P = Operands<T, C>;
@@ -323,7 +323,8 @@ void attn_tile_kernel(TileArgs a) {
   using KM = Mfma32<typename P::K>;
   using VM = Mfma32<typename P::V>;
   constexpr bool kCodes = P::kCodes;
-  constexpr int KT = F::KT, KW = F::KW, KPW = F::KPW, KB = KPW / 32, BPW = F::BPW;
+  constexpr int KT = F::KT, KW = F::KW, KPW = F::KPW, KB = KPW / F::SUB / 32,
+                BPW = F::BPW;
   constexpr int QSTEPS = D / 16, DBLK = D / 32;
   constexpr int CPR = D / E::kPer16B;             // 16-byte chunks of a cached row
   constexpr int RPL = 64 / CPR;                   // rows of a wavefront-wide load
@@ -341,7 +342,7 @@ void attn_tile_kernel(TileArgs a) {
   float* const s_sc = reinterpret_cast<float*>(s_kv + NST * 2 * TILE);
   float2* const s_ml = reinterpret_cast<float2*>(s_sc + NST * 3 * KT);   // [4][32]
   int* const s_off = reinterpret_cast<int*>(s_ml + 128);
-  __shared__ int s_part[8], s_ctx[kRankMax], s_pick;
+  __shared__ int s_part[16], s_ctx[kRankMax], s_pick;
 
   const int H = a.r.num_heads, Hkv = a.r.num_kv_heads;
   const int G = H / Hkv;
@@ -589,11 +590,12 @@ void attn_tile_kernel(TileArgs a) {
     return (uint32_t)v;
   };
 
-  auto compute = [&](int tile, int st) {
-    const int k0 = tile * KT + kg * KPW;           // this wavefront's first key
-    const uint32_t kt = (uint32_t)(2 * st * 2 * TILE + (kWide ? 4 : 2) * kg * KPW * D);
+  auto compute = [&](int tile, int st, int sub) {
+    const int off = kg * KPW + 32 * KB * sub;      // this wavefront's first key of the step
+    const int k0 = tile * KT + off;
+    const uint32_t kt = (uint32_t)(2 * st * 2 * TILE + (kWide ? 4 : 2) * off * D);
     const uint32_t vt = kt + 2 * TILE;
-    const float* const s_ks = s_sc + st * 3 * KT + kg * KPW;
+    const float* const s_ks = s_sc + st * 3 * KT + off;
     const float* const s_vs = s_ks + KT;
     // Four K operands in flight: read j + 4 goes out when product j has taken
     // its buffer (left to itself, the compiler waits out each read in turn).
@@ -666,7 +668,7 @@ void attn_tile_kernel(TileArgs a) {
       }
     }
     const int open = TREE ? U.committed : U.committed + U.row0 / G + 1;
-    if (k0 + KPW > min(open, U.kend)) {            // the same in all lanes
+    if (k0 + 32 * KB > min(open, U.kend)) {            // the same in all lanes
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         const int kk = k0 + 32 * kb;
@@ -941,7 +943,8 @@ void attn_tile_kernel(TileArgs a) {
           write_tile(i + 1, st ^ 1);
           if (i + 2 < t1) load_tile(i + 2);
         }
-        compute(i, st);
+#pragma unroll 1
+        for (int sub = 0; sub < F::SUB; ++sub) compute(i, st, sub);
         team_barrier();
       }
     } else {
@@ -951,7 +954,7 @@ void attn_tile_kernel(TileArgs a) {
         if (i + 1 < t1) load_tile(i + 1);
         if constexpr (RW > 1) team_barrier();
         else wait_lds();
-        compute(i, 0);
+        compute(i, 0, 0);
       }
     }
     finish(t, t1);
