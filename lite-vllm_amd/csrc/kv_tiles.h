@@ -1,6 +1,8 @@
 // Attention over paged caches on the matrix cores (the kernel and its launch;
 // included by one translation unit per query type).
 #pragma once
+#include <utility>
+
 #include "kv_attention.h"
 #include "lv_attn.h"
 #include "lv_mfma.h"
@@ -283,6 +285,46 @@ template <int N>
 __device__ __forceinline__ void settle(uint4 (&q)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(q[i].x), "+v"(q[i].y), "+v"(q[i].z), "+v"(q[i].w));
+}
+
+// Lane I of every 16 lanes' x, in all of them: part of the instruction that
+// takes it (DPP).
+template <int I> __device__ __forceinline__ float row_lane(float x) {
+  return __uint_as_float(
+      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x150 + I, 0xf, 0xf, true));
+}
+using Sixteen = std::make_integer_sequence<int, 16>;
+// x[i] times, plus lane i's value (not contracted to one instruction: that has
+// no DPP form).
+template <int... I>
+__device__ __forceinline__ void scale_rows(f32x16_t& x, float mul, std::integer_sequence<int, I...>) {
+#pragma clang fp contract(off)
+  ((x[I] = row_lane<I>(mul) * x[I]), ...);
+}
+template <int... I>
+__device__ __forceinline__ void add_rows(f32x16_t& x, float add, std::integer_sequence<int, I...>) {
+#pragma clang fp contract(off)
+  ((x[I] = row_lane<I>(add) + x[I]), ...);
+}
+// sum + the sum of x[i] times lane i's value.  (The compiler does not make this
+// form itself.  All lanes are on.  The first wait states are those that DPP and the results of
+// exp2 need, which it does not add before assembly.)
+__device__ __forceinline__ float sum_rows(const f32x16_t& x, float mul, float sum) {
+#define LV_FMAC(i, r) "v_fmac_f32_dpp %0, %1, %" #r " row_newbcast:" #i " row_mask:0xf bank_mask:0xf\n"
+  asm("s_nop 1\n"
+      LV_FMAC(0, 2) LV_FMAC(1, 3) LV_FMAC(2, 4) LV_FMAC(3, 5)
+      LV_FMAC(4, 6) LV_FMAC(5, 7) LV_FMAC(6, 8) LV_FMAC(7, 9)
+      : "+&v"(sum)
+      : "v"(mul), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]),
+        "v"(x[7]));
+  asm("s_nop 1\n"
+      LV_FMAC(8, 2) LV_FMAC(9, 3) LV_FMAC(10, 4) LV_FMAC(11, 5)
+      LV_FMAC(12, 6) LV_FMAC(13, 7) LV_FMAC(14, 8) LV_FMAC(15, 9)
+      : "+&v"(sum)
+      : "v"(mul), "v"(x[8]), "v"(x[9]), "v"(x[10]), "v"(x[11]), "v"(x[12]), "v"(x[13]), "v"(x[14]),
+        "v"(x[15]));
+#undef LV_FMAC
+  return sum;
 }
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -568,6 +610,9 @@ void attn_tile_kernel(TileArgs a) {
     l_run = 0.0f;
   };
 
+  // Score i of 32 keys is key 8 (i / 4) + i % 4 + 4 h; the lane that holds that
+  // key's scales for its 16 lanes is i.
+  const int own_key = 8 * ((lane & 15) >> 2) + (lane & 3) + 4 * h;
   // Byte offsets in a stage of this lane's operands: the swizzle is an XOR of
   // the chunk, so the chunk of k-step s (dim block b) is one more XOR away.
   const uint32_t k_at = 2 * (lr * D + 8 * (h ^ L::swz(lr)));      // ^ 32 s
@@ -651,17 +696,8 @@ void attn_tile_kernel(TileArgs a) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       if constexpr (kCodes) {
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const float4 ks = *reinterpret_cast<const float4*>(s_ks + 32 * kb + 8 * q4 + 4 * h);
-          float4 add = make_float4(0, 0, 0, 0);
-          if constexpr (P::kLog)
-            add = *reinterpret_cast<const float4*>(s_vs + 32 * kb + 8 * q4 + 4 * h);
-          sv[kb][4 * q4] = fmaf(sv[kb][4 * q4], ks.x, add.x);
-          sv[kb][4 * q4 + 1] = fmaf(sv[kb][4 * q4 + 1], ks.y, add.y);
-          sv[kb][4 * q4 + 2] = fmaf(sv[kb][4 * q4 + 2], ks.z, add.z);
-          sv[kb][4 * q4 + 3] = fmaf(sv[kb][4 * q4 + 3], ks.w, add.w);
-        }
+        scale_rows(sv[kb], s_ks[32 * kb + own_key], Sixteen{});
+        if constexpr (P::kLog) add_rows(sv[kb], s_vs[32 * kb + own_key], Sixteen{});
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) sv[kb][i] *= a.r.scale_log2;
@@ -715,25 +751,12 @@ void attn_tile_kernel(TileArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) sv[kb][i] = fast_exp2(sv[kb][i] - m_run);
       if constexpr (P::kLog) {
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const float4 rv = *reinterpret_cast<const float4*>(s_vs + KT + 32 * kb + 8 * q4 + 4 * h);
-          l_run = fmaf(sv[kb][4 * q4], rv.x, l_run);
-          l_run = fmaf(sv[kb][4 * q4 + 1], rv.y, l_run);
-          l_run = fmaf(sv[kb][4 * q4 + 2], rv.z, l_run);
-          l_run = fmaf(sv[kb][4 * q4 + 3], rv.w, l_run);
-        }
+        l_run = sum_rows(sv[kb], s_vs[KT + 32 * kb + own_key], l_run);
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) l_run += sv[kb][i];
-        if constexpr (kCodes) {
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            const float4 vs = *reinterpret_cast<const float4*>(s_vs + 32 * kb + 8 * q4 + 4 * h);
-            sv[kb][4 * q4] *= vs.x; sv[kb][4 * q4 + 1] *= vs.y;
-            sv[kb][4 * q4 + 2] *= vs.z; sv[kb][4 * q4 + 3] *= vs.w;
-          }
-        }
+        if constexpr (kCodes)
+          scale_rows(sv[kb], s_vs[32 * kb + own_key], Sixteen{});
       }
       if constexpr (kWide) {
         // a step of two keys: 8 q4 + e from half h = 0, 4 more from h = 1, as
