@@ -101,7 +101,8 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
     p.direct = 0;
     p.slot_heads = std::min(num_kv_heads, 8);
     while (num_kv_heads % p.slot_heads != 0) --p.slot_heads;
-    const int64_t list = (int64_t)n_seqs * (num_kv_heads / p.slot_heads) * ((max_blocks + 1) / 2);
+    const int64_t list = (int64_t)n_seqs * (num_kv_heads / p.slot_heads) *
+                         std::max(1, (max_blocks + 1) / 2);
     p.grid = p.ranges = (int)std::min<int64_t>(list, cus * (8 / p.slot_heads));
   }
   if (p.direct < 2) {

@@ -23,6 +23,7 @@ inline TileArgs tile_args(const Call& a, const TilePlan& p, char* ws) {
 
 template <typename T, int D>
 int launch_join(const Call& a, const TilePlan& p, const TileArgs& t) {
+  if (p.ranges < 2) return LV_OK;
   constexpr int TEAMS = 256 / (D / 4);
   // few rows may have many pieces: the teams share them
   const int rows = p.slot_heads * p.slot_rows;
@@ -38,7 +39,7 @@ int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
   const TileArgs t = tile_args(a, p, ws);
   const size_t lds = F::lds(D, Operands<T, C>::kWide ? 4 : 2) + (size_t)(p.n_seqs + 1) * 4;
   attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, F::THREADS, lds, a.stream>>>(t);
-  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct >= 2 || p.ranges < 2)
+  if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct >= 2)
     return rc;
   return launch_join<T, D>(a, p, t);
 }

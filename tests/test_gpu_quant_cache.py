@@ -365,6 +365,23 @@ def test_layouts_strides_and_rows_past_the_batch(device, layout):
     assert bool((out[32:] == 3.0).all()) and bool((out[:, [0, 7]] == 3.0).all())
 
 
+@pytest.mark.parametrize("seqs", [1, 700])
+def test_no_blocks(device, seqs):
+    """Tables without a column: no sequence has a key, every row is zeros."""
+    _say(f"no blocks {seqs}")
+    cache = ops.quant_kv_cache(1, BS, 2, 64, torch.int8, device)
+    q = torch.ones(seqs, 4, 64, dtype=torch.bfloat16, device=device)
+    tables = torch.zeros((seqs, 0), dtype=torch.int32, device=device)
+    ctx = torch.full((seqs,), 5, dtype=torch.int32, device=device)
+    cu = torch.arange(seqs + 1, dtype=torch.int32, device=device)
+    got = ops.paged_attention_quant(q, cache, tables, ctx, scale=1.0, out=torch.ones_like(q))
+    assert not got.any()
+    mask = torch.ones((seqs, 1), dtype=torch.int64, device=device)
+    got = ops.tree_attention_quant(q, cache, tables, ctx, cu, mask, scale=1.0, max_query_len=1,
+                                   out=torch.ones_like(q))
+    assert not got.any()
+
+
 def test_block_ids_outside_the_cache(device):
     _say("bad block ids")
     b = make_batch(14, device, (4, 2, 64), [40, 40], [1, 20], torch.bfloat16, torch.int8)

@@ -207,6 +207,53 @@ def test_context_shorter_than_the_rows(device):
     assert not got[10:].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("code", [None, torch.int8, torch.float8_e4m3fn])
+def test_scores_of_huge_magnitude(device, dtype, code):
+    """Scores near the end of the fp32 range: the larger one takes all, also
+    where every score is far below zero."""
+    _say(f"huge {dtype} {code}")
+    b = make_trees(34, device, (4, 2, 64), [1, 40], [1, 40], dtype, fill=0.0)
+    b["q"] = torch.full_like(b["q"], 1e18)
+    k, v = (x.cpu() for x in b["kv"])
+    k.fill_(-2e18)
+    best = []
+    for i in range(2):
+        p = int(b["ctx"][i]) - b["lens"][i]       # the first drafted token: all see it
+        at = int(b["tables"][i, p // BS]), p % BS
+        k[at] = -1e18
+        best.append(v[at])
+    b["kv"] = [k.to(device), v.to(device)]
+    if code is not None:
+        n = k.shape[0]
+        b["cache"] = ops.quant_kv_cache(n, BS, 2, 64, code, device)
+        rows_ = [x.view(n * BS, 2, 64) for x in b["kv"]]
+        ops.kv_scatter_quant(*rows_, b["cache"], torch.arange(n * BS, device=device))
+        best = [oq.values(x, code) for x in best]
+    b["sees"][1][:, 0] = True
+    assert all(s[:, 0].all() for s in b["sees"])
+    b["mask"][:, 0] |= 1
+    got = run(b, device).double().cpu()
+    for i in range(2):
+        for j in range(int(b["cu"][i]), int(b["cu"][i + 1])):
+            want = best[i].double().repeat_interleave(2, 0)
+            # weights 1 and 0: the result's rounding, and three fp32 roundings
+            # (a reciprocal of the scale, the quotient, the unit)
+            tol = (torch.finfo(dtype).eps / 2 + 4 * 2.0 ** -23) * want.abs()
+            assert bool(((got[j] - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_sequences(device, dtype):
+    """More sequences than a launch takes, one of them with several row tiles."""
+    _say(f"many trees {dtype}")
+    n = 4200
+    nodes = [1 + i % 2 for i in range(n)]
+    nodes[4150] = 70
+    b = make_trees(35, device, (4, 2, 64), [i % 5 for i in range(n)], nodes, dtype)
+    check(run(b, device), reference(b), dtype)
+
+
 def test_block_ids_outside_the_cache(device):
     _say("tree bad ids")
     b = make_trees(30, device, (4, 2, 64), [40], [10], torch.bfloat16)
