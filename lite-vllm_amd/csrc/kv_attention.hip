@@ -7,7 +7,9 @@
 // row (codes c, scale s) of a key, score and output are
 //   x_t = scale * s_t * (q . c_t),   o = sum_t w_t s'_t c'_t / sum_t w_t,
 //   w_t = exp(x_t - max)
-// with the codes taken as they are and the scales applied to fp32 values.
+// with the codes taken as they are and the scales applied to fp32 values.  The
+// kernels are in kv_tiles.h and kv_narrow.h; here are the ancestor bits, how a
+// call is split into launches, and the entry points.
 #include <algorithm>
 #include <atomic>
 
@@ -16,7 +18,8 @@
 namespace lv {
 
 // Ancestor bits: thread per drafted token walks up its parents, whose indices
-// fall, so that every walk ends.
+// fall, so that every walk ends.  Bound by the latency of that chain, one read
+// from L2 a level.
 __global__ __launch_bounds__(256) void tree_mask_kernel(const int32_t* __restrict__ parents,
                                                         const int32_t* __restrict__ cu,
                                                         int num_seqs, int num_tokens,

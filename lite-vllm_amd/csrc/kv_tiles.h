@@ -22,11 +22,15 @@ namespace lv {
 // joins them.  Where there are many units and none is long against a range, a
 // workgroup takes a whole unit instead (direct), longest sequences and last
 // rows first, so that there are no pieces: 15 chunks of 512 tokens at offsets
-// of 0-3071 (960 units) beside 192 decode rows 398 -> 369 us.
+// of 0-3071, 2 query heads for each of 8 kv heads (480 units of 256 rows),
+// beside 192 decode rows 393 -> 317 us.
 //
 // A workgroup is 4 wavefronts: RW groups of 32 rows times KW = 4 / RW parts
 // of every tile's keys, so that few rows (RW = 1: decodes, small trees) still
 // use four wavefronts; the KW states are merged through LDS when a piece ends.
+// More than 128 rows: 8 wavefronts, RW = 8, which halves what each does to
+// bring a tile into LDS (two chunks of 700-1024 tokens at 15000-19000, 8 query
+// heads a kv head: 350 us with RW = 4, 309 with 8).
 // Per tile:
 //   * the next tile's rows are loaded from HBM into registers while this one
 //     is computed, then turned into 16-bit operands (codes are exact in bf16
@@ -36,19 +40,31 @@ namespace lv {
 //   * x = S^T * (scale of the key's row * scale), masked by position or tree;
 //     maximum (raised rarely), weights and their sum in fp32;
 //   * O^T += V^T P^T with P = weight * scale of the value's row.
+// The scales of a score's keys come from LDS as one register, 16 lanes holding
+// 16 keys, and by DPP into the instruction that takes them: read as they lie
+// for 16 keys (b128, the same for 32 lanes) they were most of the LDS time (the
+// chunks above 309 -> 292 us, trees of 25-60 tokens at 2000-16000 213 -> 198).
+//
 // P would lose 2^-9 of each weight as bf16, an error as large as that of a
-// bf16 output.  16-bit queries over codes: P is one fp16 value (2^-12).  With
+// bf16 output.  16-bit queries over codes: P is one fp16 value (2^-11).  With
 // y = x + log2(scale of the value's row), P = exp2(y - reference) takes no
 // multiplication, the weights' sum is sum P / scale, and the reference follows
 // the largest y, so that the largest P of a row is between 2^10 and 2^15
-// whatever the scales are.  (Against two bf16 parts, 48 products a tile instead
-// of 32 and 12 vector instructions a score instead of 9: 462 -> 390 us
-// for two chunks of 700-1024 tokens at 15000-19000, 8 query heads a kv head.)
+// whatever the scales are.  (Two bf16 parts take 48 products a tile instead of
+// 32 and 12 vector instructions a score instead of 9: 462 us for the chunks
+// above against 390 when both were measured.)
 // Scales outside [2^-60, 2^20] of the unit's first ones, and ones that are not
 // finite, make the piece careful (below).  fp32 queries: three bf16 parts, all
 // the bits.  A bf16 cache: two (2^-17), an fp16 cache: one fp16 value.
 // fp32 queries are three bf16 parts (all their bits), others are taken as
-// they are.
+// they are.  An fp32 cache keeps fp32 operands and v_mfma_f32_32x32x2 (157
+// TFLOP/s at most; six products of bf16 parts would need three times the LDS):
+// trees of 40-64 tokens at 500-4000, 48 sequences, 8 kv heads of 128: 594 us.
+//
+// What bounds it: over a 16-bit cache HBM, 130 us for those trees in bf16
+// (3.6 TB/s); the chunks above at 292 us the issue of one SIMD's two wavefronts
+// (registers allow no third), whose products (40% of the time) and vector
+// instructions (65%) overlap little.
 //
 // Zero weights times a value that is not finite make NaN: a piece whose sums
 // are not finite is computed again key by key (careful), where a key that a
