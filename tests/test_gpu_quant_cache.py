@@ -439,6 +439,7 @@ def test_cache_past_32_bit_offsets(device):
     check(got, [torch.cat(x) for x in zip(*outs)], torch.bfloat16)
 
 
+@torch.inference_mode()
 def test_streams_and_graphs(device):
     """On another stream; and two captured graphs replayed in turn with eager
     work between, each owning its workspace."""

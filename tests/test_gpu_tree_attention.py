@@ -286,6 +286,7 @@ def test_mask_of_parents(device):
         assert np.array_equal(got.cpu().numpy(), want)
 
 
+@torch.inference_mode()
 def test_streams_and_graphs(device):
     _say("tree streams and graphs")
     a = make_trees(31, device, (16, 8, 128), [2000, 90], [20, 64], torch.bfloat16)
