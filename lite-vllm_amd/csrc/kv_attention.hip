@@ -80,12 +80,12 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   p.max_q = max_q;
   const int64_t rows = std::max<int64_t>(1, (int64_t)max_q * (num_heads / num_kv_heads));
   p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || dtype == LV_F32 ? 4 : 8;
-  const int r = 32 * p.rw, kt = p.rw == 4 ? 64 : 128;
+  const int r = 32 * p.rw, kt = p.rw == 4 && dtype == LV_F32 ? 64 : 128;
   const int64_t units = (int64_t)n_seqs * num_kv_heads * ((rows + r - 1) / r);
   const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_blocks * kBs + kt - 1) / kt);
   const int64_t cus = device_cus();
   p.nq = (int)((rows + r - 1) / r);
-  const int64_t at_once = cus * (dtype == LV_F32 || p.rw == 8 ? 1 : 2);
+  const int64_t at_once = cus * (dtype == LV_F32 || p.rw > 1 ? 1 : 2);
   p.ranges = (int)std::min<int64_t>(units * tiles, at_once);
   p.grid = p.ranges;
   const bool one_round = units <= at_once;

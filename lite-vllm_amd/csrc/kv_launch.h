@@ -35,7 +35,7 @@ int launch_join(const Call& a, const TilePlan& p, const TileArgs& t) {
 
 template <typename T, typename C, int D, int RW, bool TREE>
 int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
-  using F = TileCfg<RW>;
+  using F = TileCfg<RW, std::is_same<T, float>::value>;
   const TileArgs t = tile_args(a, p, ws);
   const size_t lds = F::lds(D, Operands<T, C>::kWide ? 4 : 2) + (size_t)(p.n_seqs + 1) * 4;
   attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, F::THREADS, lds, a.stream>>>(t);

@@ -97,16 +97,16 @@ __device__ __forceinline__ void make_uniform(Unit& u) {
   u.row0 = uniform(u.row0); u.ntiles = uniform(u.ntiles);
 }
 
-template <int RW> struct TileCfg {
-  static constexpr int WAVES = RW == 8 ? 8 : 4, THREADS = 64 * WAVES;
+template <int RW, bool F32> struct TileCfg {
+  static constexpr int WAVES = RW > 1 && !F32 ? 8 : 4, THREADS = 64 * WAVES;
   static constexpr int R = 32 * RW, KW = WAVES / RW;
-  static constexpr int KT = RW == 4 ? 64 : 128;   // keys per tile
+  static constexpr int KT = RW == 4 && F32 ? 64 : 128;   // keys per tile
   static constexpr int BPW = KT / (16 * WAVES);   // 16-token blocks a wavefront stages
   static constexpr int KPW = KT / KW;             // keys a wavefront computes
   static constexpr int SUB = KPW > 64 ? 2 : 1;    // in so many steps
-  static constexpr int NST = RW >= 4 ? 2 : 1;     // LDS stages
+  static constexpr int NST = RW >= (F32 ? 4 : 2) ? 2 : 1;     // LDS stages
   static constexpr size_t lds(int d, int bytes) { // operands of so many bytes; without the
-    return (size_t)NST * (KT * d * 2 * bytes + KT * 12) + 128 * 8;      // list's offsets
+    return (size_t)NST * (KT * d * 2 * bytes + KT * 12) + 32 * WAVES * 8;      // list's offsets
   }
 };
 
@@ -122,9 +122,8 @@ __device__ __forceinline__ Seq tile_sequence(const TileArgs& a, int i) {
 }
 
 // Tiles of sequence i, over all its row tiles and kv heads.
-template <bool TREE, int RW>
+template <bool TREE, typename F>
 __device__ __forceinline__ int sequence_tiles(const TileArgs& a, const Seq& s, int g) {
-  using F = TileCfg<RW>;
   const int rows = min(s.n, a.max_q) * g;
   int sum = 0;
   if (TREE) {
@@ -138,9 +137,8 @@ __device__ __forceinline__ int sequence_tiles(const TileArgs& a, const Seq& s, i
 
 // Exclusive scan of the sequences' tiles into off[0 .. n_seqs]; returns the
 // longest unit's tiles.
-template <bool TREE, int RW>
+template <bool TREE, typename F>
 __device__ int scan_tiles(const TileArgs& a, int g, int* off, int* part) {
-  using F = TileCfg<RW>;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int per = (a.n_seqs + F::THREADS - 1) / F::THREADS;
   const int lo = min(a.n_seqs, t * per), hi = min(a.n_seqs, lo + per);
@@ -148,7 +146,7 @@ __device__ int scan_tiles(const TileArgs& a, int g, int* off, int* part) {
   for (int i = lo; i < hi; ++i) {
     off[i] = sum;                       // within the thread's run
     const Seq s = tile_sequence(a, i);
-    sum += sequence_tiles<TREE, RW>(a, s, g);
+    sum += sequence_tiles<TREE, F>(a, s, g);
     if (s.n > 0) longest = max(longest, (s.ctx + F::KT - 1) / F::KT);
   }
   longest = (int)group_umax<64>((uint32_t)longest);
@@ -186,9 +184,8 @@ __device__ __forceinline__ int ranked_sequence(const TileArgs& a, int r, int* ct
   return *pick;
 }
 
-template <bool TREE, int RW>
+template <bool TREE, typename F>
 __device__ __forceinline__ void set_rows(const TileArgs& a, Unit& u, int ctx, int g) {
-  using F = TileCfg<RW>;
   u.kend = keys_needed<TREE, F::R>(ctx, u.committed, u.rows, u.row0, g);
   u.ntiles = max(1, (u.kend + F::KT - 1) / F::KT);
 }
@@ -201,9 +198,8 @@ __device__ __forceinline__ int set_seq(const TileArgs& a, Unit& u, int i, int g)
 }
 
 // The unit that holds place p of the list, and p's tile in it.
-template <bool TREE, int RW>
+template <bool TREE, typename F>
 __device__ __forceinline__ int locate(const TileArgs& a, const int* off, int p, int g, Unit& u) {
-  using F = TileCfg<RW>;
   int lo = 0, hi = a.n_seqs - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -215,16 +211,15 @@ __device__ __forceinline__ int locate(const TileArgs& a, const int* off, int p, 
   u.kvh = rem / per_head;
   rem -= u.kvh * per_head;
   for (u.row0 = 0;; u.row0 += F::R) {
-    set_rows<TREE, RW>(a, u, ctx, g);
+    set_rows<TREE, F>(a, u, ctx, g);
     if (rem < u.ntiles || u.row0 + F::R >= u.rows) break;
     rem -= u.ntiles;
   }
   return rem;
 }
 
-template <bool TREE, int RW>
+template <bool TREE, typename F>
 __device__ __forceinline__ Unit next_unit(const TileArgs& a, Unit u, int g) {
-  using F = TileCfg<RW>;
   u.row0 += F::R;
   int ctx = u.committed + u.n;
   if (u.row0 >= u.rows) {
@@ -234,7 +229,7 @@ __device__ __forceinline__ Unit next_unit(const TileArgs& a, Unit u, int g) {
       do ctx = set_seq(a, u, u.seq + 1, g); while (u.rows == 0 && u.seq + 1 < a.n_seqs);
     }
   }
-  set_rows<TREE, RW>(a, u, ctx, g);
+  set_rows<TREE, F>(a, u, ctx, g);
   return u;
 }
 
@@ -371,10 +366,13 @@ template <typename T, typename C> struct Operands {
 // Wavefronts per SIMD: the three parts of fp32 queries need the registers of two.
 template <typename T> constexpr int kTileWaves = std::is_same<T, float>::value ? 1 : 2;
 
+template <typename T, int RW>
+constexpr int kTileThreads = TileCfg<RW, std::is_same<T, float>::value>::THREADS;
+
 template <typename T, typename C, int D, int RW, bool TREE>
-__global__ __launch_bounds__(TileCfg<RW>::THREADS, kTileWaves<T>)
+__global__ __launch_bounds__((kTileThreads<T, RW>), kTileWaves<T>)
 void attn_tile_kernel(TileArgs a) {
-  using F = TileCfg<RW>;
+  using F = TileCfg<RW, std::is_same<T, float>::value>;
   using P = Operands<T, C>;
   using E = cached<C>;
   using L = ChunkLds<D, 4>;
@@ -398,8 +396,8 @@ void attn_tile_kernel(TileArgs a) {
   uint16_t* const s_kv = reinterpret_cast<uint16_t*>(s_dyn);       // [NST][K, V][TILE]
   // [NST][KT] each: K's scales; V's scales, or their logarithms and inverses
   float* const s_sc = reinterpret_cast<float*>(s_kv + NST * 2 * TILE);
-  float2* const s_ml = reinterpret_cast<float2*>(s_sc + NST * 3 * KT);   // [4][32]
-  int* const s_off = reinterpret_cast<int*>(s_ml + 128);
+  float2* const s_ml = reinterpret_cast<float2*>(s_sc + NST * 3 * KT);   // [WAVES][32]
+  int* const s_off = reinterpret_cast<int*>(s_ml + 32 * F::WAVES);
   __shared__ int s_part[16], s_ctx[kRankMax], s_pick;
 
   const int H = a.r.num_heads, Hkv = a.r.num_kv_heads;
@@ -412,7 +410,7 @@ void attn_tile_kernel(TileArgs a) {
   int r0 = 0, r1 = 1, w = 0, t = 0, per = 1;
   bool direct = a.direct >= 2;
   if (!direct) {
-    const int longest = uniform(scan_tiles<TREE, RW>(a, G, s_off, s_part));
+    const int longest = uniform(scan_tiles<TREE, F>(a, G, s_off, s_part));
     const int total = uniform(s_off[a.n_seqs]);
     per = max(1, (int)(((int64_t)total + a.ranges - 1) / a.ranges));
     direct = a.direct == 1 && longest <= 2 * per;
@@ -438,10 +436,10 @@ void attn_tile_kernel(TileArgs a) {
     U.kvh = grp % Hkv;
     U.row0 = (a.nq - 1 - slot % a.nq) * F::R;
     if (U.row0 >= U.rows) return;
-    set_rows<TREE, RW>(a, U, ctx, G);
+    set_rows<TREE, F>(a, U, ctx, G);
     make_uniform(U);
   } else {
-    t = uniform(locate<TREE, RW>(a, s_off, r0, G, U));
+    t = uniform(locate<TREE, F>(a, s_off, r0, G, U));
     make_uniform(U);
     if (t > 0 && threadIdx.x == 0) {
       // the range starts inside a unit; if that unit starts in the range
@@ -921,7 +919,7 @@ void attn_tile_kernel(TileArgs a) {
               o[b][4 * q4 + 2] * inv, o[b][4 * q4 + 3] * inv);
     } else {
       constexpr int GRP = DBLK * 4 / KW;           // groups of four dims each wavefront ends with
-      float4* const xo = reinterpret_cast<float4*>(s_dyn);     // [4][DBLK * 4][64]
+      float4* const xo = reinterpret_cast<float4*>(s_dyn);     // [WAVES][DBLK * 4][64]
       team_barrier();                              // nobody reads the tiles any more
 #pragma unroll
       for (int b = 0; b < DBLK; ++b)
@@ -1004,7 +1002,7 @@ void attn_tile_kernel(TileArgs a) {
     finish(t, t1);
     p += t1 - t;
     if (direct || p >= r1) break;
-    U = next_unit<TREE, RW>(a, U, G);
+    U = next_unit<TREE, F>(a, U, G);
     make_uniform(U);
     t = 0;
   }
