@@ -84,6 +84,7 @@ struct Call {
 struct TilePlan {
   int seq_begin, n_seqs, max_q;
   int rw;                   // tile kernel: 32-row groups of a unit, 1, 2, 4 or 8; 0: narrow kernel
+  int waves;                // and its wavefronts
   int grid, ranges;         // workgroups; ranges that the list is split into
   int direct, nq;           // (see TileArgs)
   int slot_heads, slot_rows;

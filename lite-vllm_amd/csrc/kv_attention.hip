@@ -79,27 +79,59 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   p.n_seqs = n_seqs;
   p.max_q = max_q;
   const int64_t rows = std::max<int64_t>(1, (int64_t)max_q * (num_heads / num_kv_heads));
-  p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || dtype == LV_F32 ? 4 : 8;
-  const int r = 32 * p.rw, kt = p.rw == 4 && dtype == LV_F32 ? 64 : 128;
-  const int64_t units = (int64_t)n_seqs * num_kv_heads * ((rows + r - 1) / r);
-  const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_blocks * kBs + kt - 1) / kt);
+  const bool f32 = dtype == LV_F32;
   const int64_t cus = device_cus();
+  const int64_t groups = (int64_t)n_seqs * num_kv_heads;
+  auto units_of = [&](int r) { return groups * ((rows + r - 1) / r); };
+  p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || f32 ? 4 : 8;
+  p.waves = 4;
+  // Eight wavefronts (one workgroup a CU, two for four) pay where a workgroup
+  // stays with long rows: few units, or long contexts of codes, whose way into
+  // LDS they share.  Where there are many short units two workgroups hide each
+  // other's starts.  us with eight | four: 48 trees of 40-64 tokens at 500-4000
+  // 134 | 139, of 12-16 tokens 99 | 114, 4 trees over codes 37.5 | 45, two
+  // chunks of 700-1024 at 15000-19000 292 | 343, 60 chunks of 100 at 0-3000
+  // 140 | 159; 256 trees of 40-64 at 300-1000 323 | 228, at 1000-3000 627 | 533,
+  // 60 chunks of 100 at 0-300 54 | 47.  33-64 rows on four wavefronts are half
+  // a unit of RW = 4, since RW = 2 on four has too few registers (48 trees of
+  // 20-32 tokens at 500-4000 173, RW = 4 125, RW = 2 on eight 102).  Up to 32
+  // rows over codes stay with four (16 trees of 4-8 tokens at 2000-16000 90 |
+  // 67).  fp32 keeps to four: its registers and LDS are those of one wavefront a
+  // SIMD.
+  if (!f32) {
+    const int wide = std::max(p.rw, 2);
+    if (max_blocks > 32 && (p.rw > 1 || !codes) &&
+        ((codes && max_blocks > 128) || 2 * units_of(32 * wide) <= 3 * cus)) {
+      p.rw = wide;
+      p.waves = 8;
+    } else if (p.rw > 1) {
+      p.rw = 4;
+    }
+  }
+  const int r = 32 * p.rw, kt = p.rw == 4 && p.waves == 4 ? 64 : 128;
+  const int64_t units = units_of(r);
+  const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_blocks * kBs + kt - 1) / kt);
   p.nq = (int)((rows + r - 1) / r);
-  const int64_t at_once = cus * (dtype == LV_F32 || p.rw > 1 ? 1 : 2);
+  const int64_t at_once = cus * (f32 || p.waves == 8 ? 1 : 2);
   p.ranges = (int)std::min<int64_t>(units * tiles, at_once);
   p.grid = p.ranges;
   const bool one_round = units <= at_once;
-  const int64_t all = ((int64_t)n_seqs * num_kv_heads + kXcds - 1) / kXcds * kXcds * p.nq;
+  const int64_t all = (groups + kXcds - 1) / kXcds * kXcds * p.nq;
   if (all < (1ll << 31)) {
-    // contexts of a few tiles are not split where all units run at once (a
-    // join takes as long as two tiles or three); where there are half as many
-    // units again as run at once, the kernel looks whether they need to be
+    // Contexts of a few tiles are not split where all units run at once (a join
+    // takes as long as two tiles or three: 3 decode rows of 40-300 keys 7.9 us,
+    // split 10.6, through the narrow kernel 10.6; up to 8 tiles a tree of 700
+    // keys takes 15.0, split 13.4).  Where there are half as many units again as
+    // run at once, the kernel looks whether they need to be (15 chunks of 512
+    // at 0-3071 beside decode rows 317 us, split 393).
     p.direct = one_round && tiles <= 4 ? 3 : tiles <= 2 ? 2 : 2 * units >= 3 * p.ranges ? 1 : 0;
     if (p.direct) p.grid = (int)std::max<int64_t>(all, p.direct == 1 ? p.ranges : 0);
   }
   p.slot_heads = 1;
   p.slot_rows = (int)std::min<int64_t>(rows, r);
-  if (codes && dtype != LV_F32 && rows <= 8 && p.direct != 3) {
+  // (64 decode rows of 256-4096 keys, 8 heads a kv head: 40.6 us, as tiles 45.3;
+  // 256 of 16-2048, 2 heads: 103, as tiles 174)
+  if (codes && !f32 && rows <= 8 && p.direct != 3) {
     p.rw = 0;
     p.direct = 0;
     p.slot_heads = std::min(num_kv_heads, 8);
@@ -117,6 +149,10 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   return p;
 }
 
+// Sequences of a launch that are not decode rows, at most: the largest tiles
+// leave the LDS of a CU room for so many offsets.
+constexpr int kPartSeqs = 4096;
+
 size_t plan_bytes(const TilePlan& p) { return p.head_bytes + p.ml_bytes + p.acc_bytes; }
 
 size_t workspace_size(int num_seqs, int num_decodes, int max_query_len, int num_heads,
@@ -128,8 +164,8 @@ size_t workspace_size(int num_seqs, int num_decodes, int max_query_len, int num_
     if (num_decodes > 0)
       need = std::max(need, plan_bytes(plan_tiles(0, num_decodes, 1, num_heads, num_kv_heads,
                                                   head_dim, max_blocks, dtype, codes)));
-    if (num_seqs > num_decodes)
-      need = std::max(need, plan_bytes(plan_tiles(num_decodes, num_seqs - num_decodes,
+    for (int i = num_decodes; i < num_seqs; i += kPartSeqs)
+      need = std::max(need, plan_bytes(plan_tiles(i, std::min(kPartSeqs, num_seqs - i),
                                                   max_query_len, num_heads, num_kv_heads,
                                                   head_dim, max_blocks, dtype, codes)));
   }
@@ -150,10 +186,8 @@ int launch(const Call& a, int num_decodes, int max_query_len, void* ws) {
     const TilePlan p = plan_tiles(0, num_decodes, 1, h, hkv, a.d, mb, a.dtype, codes);
     if (const int rc = launch_part(a, p, (char*)ws); rc != LV_OK) return rc;
   }
-  // (the largest tiles leave the LDS of a CU room for so many sequences' offsets)
-  constexpr int most = 4096;
-  for (int i = num_decodes; i < a.b.num_seqs; i += most) {
-    const TilePlan p = plan_tiles(i, std::min(most, a.b.num_seqs - i), max_query_len, h, hkv, a.d,
+  for (int i = num_decodes; i < a.b.num_seqs; i += kPartSeqs) {
+    const TilePlan p = plan_tiles(i, std::min(kPartSeqs, a.b.num_seqs - i), max_query_len, h, hkv, a.d,
                                   mb, a.dtype, codes);
     if (const int rc = launch_part(a, p, (char*)ws); rc != LV_OK) return rc;
   }

@@ -33,12 +33,12 @@ int launch_join(const Call& a, const TilePlan& p, const TileArgs& t) {
   return check_launch("attn_join_kernel");
 }
 
-template <typename T, typename C, int D, int RW, bool TREE>
+template <typename T, typename C, int D, bool TREE, int RW, int WAVES>
 int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
-  using F = TileCfg<RW, std::is_same<T, float>::value>;
+  using F = TileCfg<RW, WAVES>;
   const TileArgs t = tile_args(a, p, ws);
   const size_t lds = F::lds(D, Operands<T, C>::kWide ? 4 : 2) + (size_t)(p.n_seqs + 1) * 4;
-  attn_tile_kernel<T, C, D, RW, TREE><<<(unsigned)p.grid, F::THREADS, lds, a.stream>>>(t);
+  attn_tile_kernel<T, C, D, F, TREE><<<(unsigned)p.grid, F::THREADS, lds, a.stream>>>(t);
   if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct >= 2)
     return rc;
   return launch_join<T, D>(a, p, t);
@@ -54,6 +54,19 @@ int launch_narrow_kernel(const Call& a, const TilePlan& p, char* ws) {
   return launch_join<T, D>(a, p, t);
 }
 
+template <typename T, typename C, int D, bool TREE>
+int launch_tiles_rw(const Call& a, const TilePlan& p, char* ws) {
+  if (p.rw == 1) return launch_tile_kernel<T, C, D, TREE, 1, 4>(a, p, ws);
+  if constexpr (std::is_same<T, float>::value) {
+    if (p.rw == 2) return launch_tile_kernel<T, C, D, TREE, 2, 4>(a, p, ws);
+  } else if (p.waves == 8) {
+    if (p.rw == 2) return launch_tile_kernel<T, C, D, TREE, 2, 8>(a, p, ws);
+    if (p.rw == 4) return launch_tile_kernel<T, C, D, TREE, 4, 8>(a, p, ws);
+    return launch_tile_kernel<T, C, D, TREE, 8, 8>(a, p, ws);
+  }
+  return launch_tile_kernel<T, C, D, TREE, 4, 4>(a, p, ws);
+}
+
 template <typename T, typename C, int D>
 int launch_tiles_d(const Call& a, const TilePlan& p, char* ws) {
   if constexpr (cached<C>::kCodes && !std::is_same<T, float>::value) {
@@ -61,20 +74,8 @@ int launch_tiles_d(const Call& a, const TilePlan& p, char* ws) {
       return a.tree ? launch_narrow_kernel<T, C, D, true>(a, p, ws)
                     : launch_narrow_kernel<T, C, D, false>(a, p, ws);
   }
-  if (a.tree) {
-    if (p.rw == 1) return launch_tile_kernel<T, C, D, 1, true>(a, p, ws);
-    if (p.rw == 2) return launch_tile_kernel<T, C, D, 2, true>(a, p, ws);
-    if (std::is_same<T, float>::value || p.rw == 4)
-      return launch_tile_kernel<T, C, D, 4, true>(a, p, ws);
-    return launch_tile_kernel<T, C, D, std::is_same<T, float>::value ? 4 : 8, true>(a, p, ws);
-  }
-  if constexpr (cached<C>::kCodes) {
-    if (p.rw == 1) return launch_tile_kernel<T, C, D, 1, false>(a, p, ws);
-    if (p.rw == 2) return launch_tile_kernel<T, C, D, 2, false>(a, p, ws);
-    if (std::is_same<T, float>::value || p.rw == 4)
-      return launch_tile_kernel<T, C, D, 4, false>(a, p, ws);
-    return launch_tile_kernel<T, C, D, std::is_same<T, float>::value ? 4 : 8, false>(a, p, ws);
-  }
+  if (a.tree) return launch_tiles_rw<T, C, D, true>(a, p, ws);
+  if constexpr (cached<C>::kCodes) return launch_tiles_rw<T, C, D, false>(a, p, ws);
   return LV_ERR_UNSUPPORTED;
 }
 

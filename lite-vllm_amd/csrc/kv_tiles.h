@@ -25,12 +25,11 @@ namespace lv {
 // of 0-3071, 2 query heads for each of 8 kv heads (480 units of 256 rows),
 // beside 192 decode rows 393 -> 317 us.
 //
-// A workgroup is 4 wavefronts: RW groups of 32 rows times KW = 4 / RW parts
-// of every tile's keys, so that few rows (RW = 1: decodes, small trees) still
-// use four wavefronts; the KW states are merged through LDS when a piece ends.
-// More than 128 rows: 8 wavefronts, RW = 8, which halves what each does to
-// bring a tile into LDS (two chunks of 700-1024 tokens at 15000-19000, 8 query
-// heads a kv head: 350 us with RW = 4, 309 with 8).
+// A workgroup is 4 or 8 wavefronts: RW groups of 32 rows times KW = WAVES / RW
+// parts of every tile's keys, so that few rows (RW = 1: decodes, small trees)
+// still use four wavefronts; the KW states are merged through LDS when a piece
+// ends.  Eight halve what each does to bring a tile into LDS, and the pieces
+// (the host's rule and its measurements are in plan_tiles).
 // Per tile:
 //   * the next tile's rows are loaded from HBM into registers while this one
 //     is computed, then turned into 16-bit operands (codes are exact in bf16
@@ -42,8 +41,9 @@ namespace lv {
 //   * O^T += V^T P^T with P = weight * scale of the value's row.
 // The scales of a score's keys come from LDS as one register, 16 lanes holding
 // 16 keys, and by DPP into the instruction that takes them: read as they lie
-// for 16 keys (b128, the same for 32 lanes) they were most of the LDS time (the
-// chunks above 309 -> 292 us, trees of 25-60 tokens at 2000-16000 213 -> 198).
+// for 16 keys (b128, the same for 32 lanes) they were most of the LDS time (two
+// chunks of 700-1024 tokens at 15000-19000, 8 query heads a kv head, 309 -> 292
+// us; trees of 25-60 tokens at 2000-16000 213 -> 198).
 //
 // P would lose 2^-9 of each weight as bf16, an error as large as that of a
 // bf16 output.  16-bit queries over codes: P is one fp16 value (2^-11).  With
@@ -51,8 +51,8 @@ namespace lv {
 // multiplication, the weights' sum is sum P / scale, and the reference follows
 // the largest y, so that the largest P of a row is between 2^10 and 2^15
 // whatever the scales are.  (Two bf16 parts take 48 products a tile instead of
-// 32 and 12 vector instructions a score instead of 9: 462 us for the chunks
-// above against 390 when both were measured.)
+// 32 and 12 vector instructions a score instead of 9: 462 us for those chunks
+// against 390 when both were measured.)
 // Scales outside [2^-60, 2^20] of the unit's first ones, and ones that are not
 // finite, make the piece careful (below).  fp32 queries: three bf16 parts, all
 // the bits.  A bf16 cache: two (2^-17), an fp16 cache: one fp16 value.
@@ -61,7 +61,7 @@ namespace lv {
 // TFLOP/s at most; six products of bf16 parts would need three times the LDS):
 // trees of 40-64 tokens at 500-4000, 48 sequences, 8 kv heads of 128: 594 us.
 //
-// What bounds it: over a 16-bit cache HBM, 130 us for those trees in bf16
+// What bounds it: over a 16-bit cache HBM, 131 us for those trees in bf16
 // (3.6 TB/s); the chunks above at 292 us the issue of one SIMD's two wavefronts
 // (registers allow no third), whose products (40% of the time) and vector
 // instructions (65%) overlap little.
@@ -97,14 +97,14 @@ __device__ __forceinline__ void make_uniform(Unit& u) {
   u.row0 = uniform(u.row0); u.ntiles = uniform(u.ntiles);
 }
 
-template <int RW, bool F32> struct TileCfg {
-  static constexpr int WAVES = RW > 1 && !F32 ? 8 : 4, THREADS = 64 * WAVES;
+template <int RW_, int WAVES_> struct TileCfg {
+  static constexpr int RW = RW_, WAVES = WAVES_, THREADS = 64 * WAVES;
   static constexpr int R = 32 * RW, KW = WAVES / RW;
-  static constexpr int KT = RW == 4 && F32 ? 64 : 128;   // keys per tile
+  static constexpr int KT = WAVES == 4 && RW == 4 ? 64 : 128;   // keys per tile
   static constexpr int BPW = KT / (16 * WAVES);   // 16-token blocks a wavefront stages
   static constexpr int KPW = KT / KW;             // keys a wavefront computes
   static constexpr int SUB = KPW > 64 ? 2 : 1;    // in so many steps
-  static constexpr int NST = RW >= (F32 ? 4 : 2) ? 2 : 1;     // LDS stages
+  static constexpr int NST = RW >= 4 || WAVES == 8 ? 2 : 1;     // LDS stages
   static constexpr size_t lds(int d, int bytes) { // operands of so many bytes; without the
     return (size_t)NST * (KT * d * 2 * bytes + KT * 12) + 32 * WAVES * 8;      // list's offsets
   }
@@ -366,13 +366,10 @@ template <typename T, typename C> struct Operands {
 // Wavefronts per SIMD: the three parts of fp32 queries need the registers of two.
 template <typename T> constexpr int kTileWaves = std::is_same<T, float>::value ? 1 : 2;
 
-template <typename T, int RW>
-constexpr int kTileThreads = TileCfg<RW, std::is_same<T, float>::value>::THREADS;
-
-template <typename T, typename C, int D, int RW, bool TREE>
-__global__ __launch_bounds__((kTileThreads<T, RW>), kTileWaves<T>)
+template <typename T, typename C, int D, typename F, bool TREE>
+__global__ __launch_bounds__(F::THREADS, kTileWaves<T>)
 void attn_tile_kernel(TileArgs a) {
-  using F = TileCfg<RW, std::is_same<T, float>::value>;
+  constexpr int RW = F::RW;
   using P = Operands<T, C>;
   using E = cached<C>;
   using L = ChunkLds<D, 4>;
