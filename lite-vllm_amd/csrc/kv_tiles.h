@@ -175,7 +175,7 @@ __device__ __forceinline__ int ranked_sequence(const TileArgs& a, int r, int* ct
   if (a.n_seqs > kRankMax || a.direct == 3) return r;
   const int t = threadIdx.x;
   const int mine = t < a.n_seqs ? tile_sequence(a, t).ctx : -1;
-  ctx[t] = mine;
+  if (t < kRankMax) ctx[t] = mine;
   __syncthreads();
   int before = 0;
   for (int i = 0; i < a.n_seqs; ++i) before += ctx[i] > mine || (ctx[i] == mine && i < t);

@@ -365,6 +365,19 @@ def test_layouts_strides_and_rows_past_the_batch(device, layout):
     assert bool((out[32:] == 3.0).all()) and bool((out[:, [0, 7]] == 3.0).all())
 
 
+@pytest.mark.parametrize("code,dtype", [(torch.int8, torch.bfloat16),
+                                        (torch.float8_e4m3fn, torch.float16)])
+def test_whole_units(device, code, dtype):
+    """Many sequences, none long against a workgroup's share: a workgroup takes
+    whole units, longest contexts first; few and many rows side by side."""
+    _say(f"whole units {code} {dtype}")
+    ctx = [2100 + 7 * i if i % 20 == 3 else 850 + i % 60 for i in range(200)]
+    lens = [1 + i % 3 for i in range(200)]
+    lens[7], lens[23], lens[150] = 130, 128, 129
+    b = make_batch(20, device, (2, 2, 64), ctx, lens, dtype, code)
+    check(run(b, device, 0), reference(b), dtype)
+
+
 @pytest.mark.parametrize("seqs", [1, 700])
 def test_no_blocks(device, seqs):
     """Tables without a column: no sequence has a key, every row is zeros."""
