@@ -30,8 +30,31 @@ struct QuantView {
   int64_t blk, tok, head;        // of the codes
   int64_t sblk, stok, shead;     // of the scales
   int64_t num_slots;
-  int block_size;
+  int block_size, block_shift;   // shift: log2 of the size, or -1
 };
+
+// Scatter and gather: 64-bit divisions took more instructions than the rest of a
+// row, so the workgroup divides once, in scalars, and a lane divides the small
+// rest (7872 tokens written and read back 26.2 -> 25.0 us).  The prologue, which
+// waits longer for its loads, divides: with these it took 30.0 us for 4099
+// tokens, read back, against 26.4.
+struct RowOf { int64_t token; int head_slot; };
+template <int W>
+__device__ __forceinline__ RowOf row_of(int per_token) {
+  const int64_t first = (int64_t)blockIdx.x * (kQuantThreads / W);
+  const int64_t t0 = first / per_token;
+  const unsigned rem = (unsigned)(first - t0 * per_token) + threadIdx.x / W;
+  const unsigned up = rem / (unsigned)per_token;
+  return {t0 + up, (int)(rem - up * per_token)};
+}
+
+struct SlotOf { int64_t block; int offset; };
+__device__ __forceinline__ SlotOf slot_of(const QuantView& c, int64_t slot) {
+  if (c.block_shift >= 0)
+    return {slot >> c.block_shift, (int)(slot & (c.block_size - 1))};
+  const int64_t blk = slot / c.block_size;
+  return {blk, (int)(slot - blk * c.block_size)};
+}
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* p, float* x) {
@@ -66,8 +89,8 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, const float* y) {
 
 // W = D / 8 lanes per (token, K or V, kv head): code = x / max|x| * top, the
 // exact quotient (lv_quant.h).  7872 bf16 tokens of 8 heads of 128 to e4m3:
-// 15.5 us, 49 MB at 3.1 TB/s; the exact quotients' vector instructions (about
-// 9 us) and HBM (10 us) overlap in part.  61 tokens: 3.7 us, one chain of slot,
+// 14.1 us, 49 MB at 3.5 TB/s; the exact quotients' vector instructions and HBM
+// (10 us) overlap in part.  61 tokens: 3.5 us, one chain of slot,
 // scale and store.
 template <typename T, typename C, int D, bool VEC>
 __global__ __launch_bounds__(kQuantThreads) void kv_scatter_quant_kernel(
@@ -76,10 +99,10 @@ __global__ __launch_bounds__(kQuantThreads) void kv_scatter_quant_kernel(
     int num_kv_heads) {
   constexpr int W = D / 8;
   const int i = (threadIdx.x & (W - 1)) * 8;
-  const int64_t row = ((int64_t)blockIdx.x * kQuantThreads + threadIdx.x) / W;
-  const int64_t t = row / (2 * num_kv_heads);
+  const RowOf row = row_of<W>(2 * num_kv_heads);
+  const int64_t t = row.token;
   if (t >= num_tokens) return;      // whole groups leave together (W divides 64)
-  const int hs = (int)(row - t * (2 * num_kv_heads));
+  const int hs = row.head_slot;
   const int kv = hs >= num_kv_heads, head = hs - kv * num_kv_heads;
   const int64_t slot = slots[t];
   float x[8];       // (loaded beside the slot, not after it)
@@ -90,15 +113,14 @@ __global__ __launch_bounds__(kQuantThreads) void kv_scatter_quant_kernel(
     return;
   }
   const float scale = row_scale<C, W, 8>(x);
-  const int64_t blk = slot / c.block_size;
-  const int off = (int)(slot - blk * c.block_size);
+  const auto [blk, off] = slot_of(c, slot);
   store_codes8<C>(c.code[kv] + blk * c.blk + off * c.tok + head * c.head + i, x);
   if (i == 0) c.scale[kv][blk * c.sblk + off * c.stok + head * c.shead] = scale;
 }
 
 // value = code * scale, one rounding.  Rows at slots outside the cache
-// (negative: padding) are zeros.  The same 7872 tokens read back: 12.1 us,
-// 4.0 TB/s, bound by HBM; 61 tokens: 3.3 us, bound by the chain slot, code,
+// (negative: padding) are zeros.  The same 7872 tokens read back: 11.4 us,
+// 4.3 TB/s, bound by HBM; 61 tokens: 3.0 us, bound by the chain slot, code,
 // store.
 template <typename T, typename C, int D, bool VEC>
 __global__ __launch_bounds__(kQuantThreads) void kv_gather_quant_kernel(
@@ -106,17 +128,16 @@ __global__ __launch_bounds__(kQuantThreads) void kv_gather_quant_kernel(
     T* __restrict__ key, int64_t key_stride, T* __restrict__ value, int64_t value_stride) {
   constexpr int W = D / 8;
   const int i = (threadIdx.x & (W - 1)) * 8;
-  const int64_t row = ((int64_t)blockIdx.x * kQuantThreads + threadIdx.x) / W;
-  const int64_t t = row / (2 * num_kv_heads);
+  const RowOf row = row_of<W>(2 * num_kv_heads);
+  const int64_t t = row.token;
   if (t >= num_tokens) return;
-  const int hs = (int)(row - t * (2 * num_kv_heads));
+  const int hs = row.head_slot;
   const int kv = hs >= num_kv_heads, head = hs - kv * num_kv_heads;
   const int64_t slot = slots[t];
   float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (slot >= c.num_slots && hs == 0 && i == 0) report_device_error(LV_DEVERR_SLOT);
   if (slot >= 0 && slot < c.num_slots) {
-    const int64_t blk = slot / c.block_size;
-    const int off = (int)(slot - blk * c.block_size);
+    const auto [blk, off] = slot_of(c, slot);
     const uint2 w = *reinterpret_cast<const uint2*>(c.code[kv] + blk * c.blk + off * c.tok +
                                                     head * c.head + i);
     const float scale = c.scale[kv][blk * c.sblk + off * c.stok + head * c.shead];
@@ -248,6 +269,7 @@ QuantView view_of(const lv_quant_cache* c) {
   v.blk = c->stride_block; v.tok = c->stride_token; v.head = c->stride_head;
   v.sblk = c->scale_stride_block; v.stok = c->scale_stride_token; v.shead = c->scale_stride_head;
   v.block_size = c->block_size;
+  v.block_shift = (c->block_size & (c->block_size - 1)) == 0 ? __builtin_ctz(c->block_size) : -1;
   v.num_slots = c->num_blocks * c->block_size;
   return v;
 }
