@@ -101,6 +101,28 @@ def test_scatter_and_gather(device, code, dtype, hkv, d, tokens, layout):
                                torch.nan_to_num(want.float(), nan=-7.0)), out_dtype
 
 
+@pytest.mark.parametrize("bs", [1, 12, 32])
+def test_block_sizes(device, bs):
+    """Slots of blocks of other sizes, no power of two among them."""
+    _say(f"block size {bs}")
+    g = torch.Generator().manual_seed(4)
+    n, hkv, d, tokens = -(-200 // bs), 5, 64, 150
+    k, v = (rows(g, tokens, hkv, d).to(torch.bfloat16) for _ in range(2))
+    slots = torch.randperm(n * bs, generator=g)[:tokens]
+    cache = ops.quant_kv_cache(n, bs, hkv, d, torch.int8, device)
+    ops.kv_scatter_quant(k.to(device), v.to(device), cache, slots.to(device))
+    for x, codes, scale in ((k, cache.key, cache.key_scale), (v, cache.value, cache.value_scale)):
+        c, s = oq.quantise(x, torch.int8)
+        want = torch.zeros(n * bs, hkv, d, dtype=torch.float64)
+        want[slots] = c
+        assert torch.equal(codes.cpu().double().reshape(-1, hkv, d), want)
+        assert torch.equal(scale.cpu().reshape(-1, hkv)[slots], s)
+    got = ops.kv_gather_quant(cache, slots.to(device), torch.float32)
+    for x, y in zip((k, v), got):
+        c, s = oq.quantise(x, torch.int8)
+        assert torch.equal(y.cpu(), c.float() * s[..., None])
+
+
 def test_gather_into_given_rows(device):
     """Strided outputs, unaligned rows, and slots past the cache."""
     _say("gather strided")
