@@ -422,23 +422,16 @@ def _plain(s):
 
 # -- one pass ------------------------------------------------------------------------
 
-_module = None
-
-
 def _ops():
-    """The package's ops, found on first use."""
-    global _module
-    if _module is None:
-        package = str(Path(__file__).resolve().parent.parent / "lite-vllm_amd")
-        if package not in sys.path:
-            sys.path.insert(0, package)
-        from litevllm import ops
-        _module = ops
-    return _module
+    package = str(Path(__file__).resolve().parent.parent / "lite-vllm_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from litevllm import ops
+    return ops
 
 
 def _own(s):
-    ops = _module or _ops()
+    ops = _ops()
     case = s["case"]
     if case["code"] != "none":
         cache = ops.QuantKV(*s["cache"])
