@@ -45,24 +45,31 @@ namespace lv {
 // chunks of 700-1024 tokens at 15000-19000, 8 query heads a kv head, 309 -> 292
 // us; trees of 25-60 tokens at 2000-16000 213 -> 198).
 //
-// P would lose 2^-9 of each weight as bf16, an error as large as that of a
-// bf16 output.  16-bit queries over codes: P is one fp16 value (2^-11).  With
-// y = x + log2(scale of the value's row), P = exp2(y - reference) takes no
-// multiplication, the weights' sum is sum P / scale, and the reference follows
-// the largest y, so that the largest P of a row is between 2^10 and 2^15
-// whatever the scales are.  (Two bf16 parts take 48 products a tile instead of
-// 32 and 12 vector instructions a score instead of 9: 462 us for those chunks
-// against 390 when both were measured.)
+// Weights.  A weight rounded to bf16 (2^-8) or, for an fp16 output, to fp16
+// (2^-11) errs as much as the output's own rounding does, and the keys' errors
+// do not cancel.  So P is as many 16-bit parts as leave nothing of that: two fp16
+// ones (2^-22) over codes and fp16 caches, two bf16 ones (2^-15) over a bf16
+// cache, three bf16 ones, all the bits, for fp32 queries.  (One fp16 part put fp16
+// outputs a third further from 64 bits than fp32 weights do, 2.7e-4 instead of
+// 2.1e-4, and bf16 ones half a percent, 1.664e-3 instead of 1.655e-3.  The second
+// costs 16 products a tile and an instruction a score: the chunks above 292 ->
+// 377 us and the trees over codes 195 -> 243, both fp16, the mixed step 318 -> 359,
+// bf16.)
+// Over codes, with y = x + log2(scale of the value's row), P = exp2(y - reference)
+// takes no multiplication, the weights' sum is sum P / scale, and the reference
+// follows the largest y, so that the largest P of a row is between 2^10 and 2^15
+// whatever the scales are and what fp16 cannot hold of the smallest, 2^-25, is
+// 2^-35 of it.  The sum y is rounded to the last place of the score, as the score
+// was when it was scaled: one rounding beside the D of its products.
 // Scales outside [2^-60, 2^20] of the unit's first ones, and ones that are not
-// finite, make the piece careful (below).  fp32 queries: three bf16 parts, all
-// the bits.  A bf16 cache: two (2^-17), an fp16 cache: one fp16 value.
+// finite, make the piece careful (below).
 // fp32 queries are three bf16 parts (all their bits), others are taken as
 // they are.  An fp32 cache keeps fp32 operands and v_mfma_f32_32x32x2 (157
 // TFLOP/s at most; six products of bf16 parts would need three times the LDS):
 // trees of 40-64 tokens at 500-4000, 48 sequences, 8 kv heads of 128: 594 us.
 //
 // What bounds it: over a 16-bit cache HBM, 131 us for those trees in bf16
-// (3.6 TB/s); the chunks above at 292 us the issue of one SIMD's two wavefronts
+// (3.6 TB/s); the chunks above at 377 us the issue of one SIMD's two wavefronts
 // (registers allow no third), whose products (40% of the time) and vector
 // instructions (65%) overlap little.
 //
@@ -269,7 +276,8 @@ __device__ __forceinline__ void codes_to_operands(const uint4& w, uint4* out) {
   out[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
-// Pairs of fp32 values as their leading bf16 / fp16 parts, taken off them.
+// Pairs of fp32 values as their leading bf16 / fp16 parts, taken off them unless
+// they are the last.
 template <typename O>
 __device__ __forceinline__ uint32_t take_part(float& a, float& b, bool last) {
   if constexpr (std::is_same<O, bf16>::value) {
@@ -287,6 +295,17 @@ __device__ __forceinline__ uint32_t take_part(float& a, float& b, bool last) {
     }
     return w;
   }
+}
+
+// The same for a leading fp16 part w and all that it leaves, as fp16: one
+// instruction a value (v_fma_mix, which the compiler does not make of a
+// difference).
+__device__ __forceinline__ uint32_t rest_of(uint32_t w, float a, float b) {
+  float minus = -1.0f;
+  asm("" : "+s"(minus));
+  const f16x2_t h = __builtin_bit_cast(f16x2_t, w);
+  const f16x2_t r = {(_Float16)fmaf((float)h[0], minus, a), (_Float16)fmaf((float)h[1], minus, b)};
+  return __builtin_bit_cast(uint32_t, r);
 }
 
 // Waits here for the loads of these registers.  Left alone, the compiler waits
@@ -353,8 +372,8 @@ template <typename T, typename C> struct Operands {
   static constexpr bool kLog = kCodes && !kF32;   // P = exp2(x + log2 of V's scale)
   using V = typename std::conditional<kCodes, typename std::conditional<kF32, bf16, f16>::type,
                                       K>::type;
-  static constexpr int QP = kF32 ? 3 : 1;
-  static constexpr int PP = kF32 ? 3 : std::is_same<V, f16>::value ? 1 : 2;
+  static constexpr int QP = kF32 ? 3 : 1;    // parts of a query, of a weight
+  static constexpr int PP = kF32 ? 3 : 2;
   static constexpr bool kWide = std::is_same<C, float>::value;   // fp32 operands
   // A row's reference is set kLift (in log2 units) under the score that sets it
   // and again when a score passes it by kTop: fp16 weights then lie high enough
@@ -790,9 +809,13 @@ void attn_tile_kernel(TileArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float x = sv[kb][2 * i], y = sv[kb][2 * i + 1];
-          pw[p][i] = take_part<typename P::V>(x, y, p + 1 == P::PP);
-          sv[kb][2 * i] = x;
-          sv[kb][2 * i + 1] = y;
+          if constexpr (P::PP == 2 && std::is_same<typename P::V, f16>::value) {
+            pw[p][i] = p == 0 ? take_part<f16>(x, y, true) : rest_of(pw[0][i], x, y);
+          } else {
+            pw[p][i] = take_part<typename P::V>(x, y, p + 1 == P::PP);
+            sv[kb][2 * i] = x;
+            sv[kb][2 * i + 1] = y;
+          }
         }
       // Each step's V operands are read while the step before is multiplied.
 #pragma unroll

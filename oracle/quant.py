@@ -101,10 +101,11 @@ def tolerance(out, spread, reach, floor, dtype: torch.dtype):
     in fp32 is off by at most (D + 4) 2^-24 of its reach (products, sums, and
     the scale's roundings), the weight by that relative amount, twice over
     through the sum of the weights; exp2 and the sums of weights and products
-    add at most 2^-20 for the lengths tested.  For 16-bit types each weight may
-    be rounded to fp16 in the numerator (the sum takes it unrounded): half a
-    step of a value of 11 significant bits is 2^-11 of it where it is largest,
-    just above a power of two (1 + 2^-11 lies between 1 and 1 + 2^-10).
+    add at most 2^-20 for the lengths tested.
+    16-bit types: the numerator may take each weight in two parts (the sum takes
+    it unrounded).  Two bf16 parts, the first cut off after 8 significant bits,
+    leave less than 2^-7 of it, which 8 bits again hold to 2^-8 of that: 2^-15.
+    Two fp16 parts, rounded, are off by 2^-11 of 2^-11.
     The smallest step of fp16 is 2^-24 whatever the value: with a row's largest
     numerator weight held at 2^10 or more a weight is off by up to half of it,
     2^-35 of the largest, so the sum by 2^-35 of the largest times the sum of
@@ -114,7 +115,7 @@ def tolerance(out, spread, reach, floor, dtype: torch.dtype):
     fixed = 0.0
     rel = 2 * (out.shape[-1] + 4) * 2.0 ** -24 * reach[..., None] + 2.0 ** -20
     if dtype != torch.float32:
-        rel = rel + 2.0 ** -11
+        rel = rel + 2.0 ** -15
         fixed = 2.0 ** -35 * floor[..., None]
     tiny = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}
     return half * out.abs() + (1 + half) * (rel * spread + fixed) + tiny[dtype]
