@@ -79,6 +79,12 @@ struct Call {
   hipStream_t stream;
 };
 
+// Sequences of a launch, at most.  A kernel keeps their offsets in LDS beside its
+// tiles: for so many the largest tiles leave room (kv_launch.h asserts it).
+constexpr int kPartSeqs = 4096;
+constexpr size_t kOffsetBytes = (size_t)(kPartSeqs + 1) * 4;
+constexpr size_t kLdsBytes = 160 * 1024;
+
 // The sequences [seq_begin, seq_begin + n_seqs) of a call, max_q rows each at
 // most: their kernel, its launch and its workspace.
 struct TilePlan {

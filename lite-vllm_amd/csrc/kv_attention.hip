@@ -149,26 +149,35 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   return p;
 }
 
-// Sequences of a launch that are not decode rows, at most: the largest tiles
-// leave the LDS of a CU room for so many offsets.
-constexpr int kPartSeqs = 4096;
-
 size_t plan_bytes(const TilePlan& p) { return p.head_bytes + p.ml_bytes + p.acc_bytes; }
+
+// The parts of a call, one launch (and its join) each: its decode rows, then its
+// other sequences, kPartSeqs at a time.  f(plan) until one does not return LV_OK.
+template <typename F>
+int for_each_part(int num_seqs, int num_decodes, int max_query_len, int num_heads,
+                  int num_kv_heads, int head_dim, int max_blocks, lv_dtype dtype, bool codes, F f) {
+  for (int i = 0, n; i < num_seqs; i += n) {
+    const bool decodes = i < num_decodes;
+    n = std::min(kPartSeqs, (decodes ? num_decodes : num_seqs) - i);
+    if (const int rc = f(plan_tiles(i, n, decodes ? 1 : max_query_len, num_heads, num_kv_heads,
+                                    head_dim, max_blocks, dtype, codes));
+        rc != LV_OK)
+      return rc;
+  }
+  return LV_OK;
+}
 
 size_t workspace_size(int num_seqs, int num_decodes, int max_query_len, int num_heads,
                       int num_kv_heads, int head_dim, int max_blocks, lv_dtype dtype) {
   // (of an 8-bit cache or not: the larger need)
   if (num_seqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || max_blocks < 0) return 0;
   size_t need = 0;
-  for (const bool codes : {false, true}) {
-    if (num_decodes > 0)
-      need = std::max(need, plan_bytes(plan_tiles(0, num_decodes, 1, num_heads, num_kv_heads,
-                                                  head_dim, max_blocks, dtype, codes)));
-    for (int i = num_decodes; i < num_seqs; i += kPartSeqs)
-      need = std::max(need, plan_bytes(plan_tiles(i, std::min(kPartSeqs, num_seqs - i),
-                                                  max_query_len, num_heads, num_kv_heads,
-                                                  head_dim, max_blocks, dtype, codes)));
-  }
+  for (const bool codes : {false, true})
+    for_each_part(num_seqs, num_decodes, max_query_len, num_heads, num_kv_heads, head_dim,
+                  max_blocks, dtype, codes, [&](const TilePlan& p) {
+                    need = std::max(need, plan_bytes(p));
+                    return LV_OK;
+                  });
   return need;
 }
 
@@ -179,19 +188,11 @@ int launch_part(const Call& a, const TilePlan& p, char* ws) {
 }
 
 int launch(const Call& a, int num_decodes, int max_query_len, void* ws) {
-  const int h = a.r.num_heads, hkv = a.r.num_kv_heads, mb = a.b.max_blocks;
   // (the narrow kernel's offsets within a block are 32 bits wide)
   const bool codes = a.code >= 0 && a.c.tok <= (1 << 26);
-  if (num_decodes > 0) {
-    const TilePlan p = plan_tiles(0, num_decodes, 1, h, hkv, a.d, mb, a.dtype, codes);
-    if (const int rc = launch_part(a, p, (char*)ws); rc != LV_OK) return rc;
-  }
-  for (int i = num_decodes; i < a.b.num_seqs; i += kPartSeqs) {
-    const TilePlan p = plan_tiles(i, std::min(kPartSeqs, a.b.num_seqs - i), max_query_len, h, hkv, a.d,
-                                  mb, a.dtype, codes);
-    if (const int rc = launch_part(a, p, (char*)ws); rc != LV_OK) return rc;
-  }
-  return LV_OK;
+  return for_each_part(a.b.num_seqs, num_decodes, max_query_len, a.r.num_heads, a.r.num_kv_heads,
+                       a.d, a.b.max_blocks, a.dtype, codes,
+                       [&](const TilePlan& p) { return launch_part(a, p, (char*)ws); });
 }
 
 // The checks common to the attention entries; fills `a` but for the cache.

@@ -37,7 +37,9 @@ template <typename T, typename C, int D, bool TREE, int RW, int WAVES>
 int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
   using F = TileCfg<RW, WAVES>;
   const TileArgs t = tile_args(a, p, ws);
-  const size_t lds = F::lds(D, Operands<T, C>::kWide ? 4 : 2) + (size_t)(p.n_seqs + 1) * 4;
+  constexpr size_t tiles = F::lds(D, Operands<T, C>::kWide ? 4 : 2);
+  static_assert(tiles + kOffsetBytes + kTileStaticLds <= kLdsBytes, "LDS of a CU");
+  const size_t lds = tiles + (size_t)(p.n_seqs + 1) * 4;
   attn_tile_kernel<T, C, D, F, TREE><<<(unsigned)p.grid, F::THREADS, lds, a.stream>>>(t);
   if (const int rc = check_launch("attn_tile_kernel"); rc != LV_OK || p.direct >= 2)
     return rc;
@@ -47,6 +49,8 @@ int launch_tile_kernel(const Call& a, const TilePlan& p, char* ws) {
 template <typename T, typename C, int D, bool TREE>
 int launch_narrow_kernel(const Call& a, const TilePlan& p, char* ws) {
   const TileArgs t = tile_args(a, p, ws);
+  static_assert(kNarrowWaves * 2 * NarrowStage<D>::BYTES + kOffsetBytes + kNarrowWaves * 4 <=
+                    kLdsBytes, "LDS of a CU");
   const size_t lds = (size_t)p.slot_heads * 2 * NarrowStage<D>::BYTES + (size_t)(p.n_seqs + 1) * 4;
   attn_narrow_kernel<T, C, D, TREE>
       <<<(unsigned)p.grid, (unsigned)(64 * p.slot_heads), lds, a.stream>>>(t);

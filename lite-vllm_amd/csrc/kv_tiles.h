@@ -382,6 +382,9 @@ template <typename T, typename C> struct Operands {
   static constexpr float kTop = std::is_same<V, f16>::value ? 15.0f : 8.0f;
 };
 
+// What the tile kernel has in LDS besides its tiles and offsets.
+constexpr size_t kTileStaticLds = (16 + kRankMax + 4) * sizeof(int);
+
 // Wavefronts per SIMD: the three parts of fp32 queries need the registers of two.
 template <typename T> constexpr int kTileWaves = std::is_same<T, float>::value ? 1 : 2;
 

@@ -525,3 +525,50 @@ def test_same_call_same_bits(device):
     first = run(b, device, 2)
     for _ in range(3):
         assert same(run(b, device, 2), first)
+
+
+@pytest.mark.parametrize("heads,dtype,width", [
+    ((16, 8, 128), torch.bfloat16, 6),        # a wavefront a kv head, the largest stages
+    ((4, 2, 64), torch.float16, 6),
+    ((8, 8, 128), torch.float32, 6),          # 32-row tiles
+    ((40, 1, 128), torch.bfloat16, 130)])     # tiles of two stages and eight wavefronts
+def test_many_decode_rows(device, heads, dtype, width):
+    """More decode rows than a launch takes, whose offsets would not fit the LDS
+    beside the tiles; other sequences behind them."""
+    _say(f"many decode rows {heads} {dtype} {width}")
+    H, Hkv, D = heads
+    n, pool = 8300, 64
+    g = torch.Generator().manual_seed(21)
+    cache = ops.quant_kv_cache(pool, BS, Hkv, D, torch.int8, device)
+    k, v = rows(g, pool * BS, Hkv, D), rows(g, pool * BS, Hkv, D)
+    ops.kv_scatter_quant(k.to(device), v.to(device), cache, torch.arange(pool * BS, device=device))
+    edges = [0, 1, 4094, 4095, 4096, 4097, 8190, 8191, 8192, 8193, n - 2, n - 1]
+    ctx = torch.randint(0, 33, (n,), generator=g, dtype=torch.int32)       # one tile
+    ctx[edges] = 16 * width - 3 if width < 100 else 700
+    lens = [1] * n
+    lens[n - 1] = 9
+    tables = torch.randint(0, pool, (n, width), generator=g, dtype=torch.int32)
+    b = dict(cache=cache, tables=tables, ctx=ctx, lens=lens, scale=1 / math.sqrt(D), heads=heads,
+             cu=torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32),
+             q=torch.randn(n + 8, H, D, generator=g).to(dtype))
+    got = run(b, device, n - 1)
+    some = edges
+    at = [r for i in some for r in range(int(b["cu"][i]), int(b["cu"][i + 1]))]
+    part = dict(b, tables=tables[some], ctx=ctx[some], lens=[lens[i] for i in some], q=b["q"][at])
+    part["cu"] = torch.tensor([0] + list(np.cumsum(part["lens"])), dtype=torch.int32)
+    check(got[at], reference(part), dtype)
+    # the others, of up to two blocks, side by side
+    kv = cache_values(cache)
+    for lo in range(0, n - 1, 1000):
+        i = torch.tensor([i for i in range(lo, min(lo + 1000, n)) if i not in edges])
+        kk, vv = (x[tables[i, :2].long()].reshape(len(i), 2 * BS, Hkv, D).transpose(1, 2) for x in kv)
+        q = b["q"][i].double().view(len(i), Hkv, H // Hkv, D)
+        sees = (torch.arange(2 * BS) < ctx[i, None])[:, None, None]        # [n, 1, 1, keys]
+        x = (q @ kk.transpose(2, 3) * b["scale"]).masked_fill(~sees, -math.inf)
+        w = torch.nan_to_num(torch.softmax(x, -1))                         # no key: zeros
+        shown = vv.abs() * sees[:, 0, 0, None, :, None]
+        reach = (b["scale"] * (q.abs() @ kk.abs().transpose(2, 3)) * sees).amax(-1)
+        floor = (ctx[i, None] * shown.amax((2, 3)))[..., None].expand_as(reach)
+        ref = [t.reshape(len(i), H, -1) for t in (w @ vv, w @ vv.abs())] \
+            + [t.reshape(len(i), H) for t in (reach, floor)]
+        check(got[i.to(device)], ref, dtype)
