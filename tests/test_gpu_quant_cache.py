@@ -400,6 +400,40 @@ def test_whole_units(device, code, dtype):
     check(run(b, device, 0), reference(b), dtype)
 
 
+def pieces_written(call, need):
+    """Runs call(workspace) and tells whether any piece of a unit went to the
+    workspace (behind its first part, 32 bytes for each of up to 512 ranges)."""
+    ws = torch.full((need,), 0x5A, dtype=torch.uint8, device="cuda")
+    call(ws)
+    return bool((ws[512 * 32:] != 0x5A).any())
+
+
+@pytest.mark.parametrize("code,dtype", [(torch.int8, torch.bfloat16),
+                                        (torch.float8_e4m3fn, torch.float16),
+                                        (torch.int8, torch.float32)])
+@pytest.mark.parametrize("longest,whole", [(1540, True), (6000, False)])
+@pytest.mark.parametrize("n", [200, 300])
+def test_units_whole_or_in_pieces(device, code, dtype, longest, whole, n):
+    """The two sides of what the kernel finds in the contexts: none is long against
+    a workgroup's share, and every unit is one workgroup's (of eight wavefronts for
+    16-bit queries), or one is, and units are split.  300 sequences are too many to
+    rank."""
+    _say(f"units {code} {dtype} {longest} {n}")
+    ctx = [1440 + 10 * (i // 20) if i % 20 == 3 else 850 + i % 60 for i in range(n)]
+    ctx[43] = longest
+    lens = [1 + i % 3 for i in range(n)]
+    lens[7], lens[23], lens[150], lens[31] = 130, 128, 129, 0
+    heads = (2, 2, 64)
+    b = make_batch(20, device, heads, ctx, lens, dtype, code)
+    # tables wider than the longest context, as a graph's are
+    b["tables"] = torch.nn.functional.pad(b["tables"], (0, 400 - b["tables"].shape[1]))
+    need = ops.paged_attention_quant_workspace_size(n, 0, sum(lens), 130, *heads, 400, dtype)
+    got = []
+    split = pieces_written(lambda ws: got.append(run(b, device, 0, workspace=ws)), need)
+    assert split != whole
+    check(got[0], reference(b), dtype)
+
+
 @pytest.mark.parametrize("seqs", [1, 700])
 def test_no_blocks(device, seqs):
     """Tables without a column: no sequence has a key, every row is zeros."""

@@ -11,7 +11,8 @@ import torch
 
 from litevllm import _hip, ops
 from oracle import quant as oq
-from test_gpu_quant_cache import BS, CODES, DTYPES, cache_values, check, make_batch, rows, same
+from test_gpu_quant_cache import (BS, CODES, DTYPES, cache_values, check, make_batch,
+                                  pieces_written, rows, same)
 
 pytestmark = pytest.mark.gpu
 
@@ -333,3 +334,25 @@ def test_same_call_same_bits(device):
     first = run(b, device)
     for _ in range(3):
         assert same(run(b, device), first)
+
+
+@pytest.mark.parametrize("code,dtype,n", [
+    (None, torch.bfloat16, 192), (None, torch.float16, 420), (torch.int8, torch.bfloat16, 200),
+    (torch.float8_e4m3fn, torch.float16, 300), (None, torch.float32, 200)])
+@pytest.mark.parametrize("longest,whole", [(1540, True), (6000, False)])
+def test_units_whole_or_in_pieces(device, code, dtype, n, longest, whole):
+    """Trees on both sides of the same choice: few and many, on eight and on four
+    wavefronts."""
+    _say(f"tree units {code} {dtype} {n} {longest}")
+    heads = (2, 2, 64)
+    offs = [1440 + 10 * (i // 50) if i % 20 == 3 else 850 + i % 60 for i in range(n)]
+    offs[43] = longest
+    nodes = [1 + i % 3 for i in range(n)]
+    nodes[7], nodes[23], nodes[150], nodes[31] = 70, 66, 130, 0
+    b = make_trees(36, device, heads, offs, nodes, dtype, code, fill=0.0)
+    b["tables"] = torch.nn.functional.pad(b["tables"], (0, 400 - b["tables"].shape[1]))
+    need = ops.tree_attention_workspace_size(n, sum(nodes), 130, *heads, 400, dtype)
+    got = []
+    split = pieces_written(lambda ws: got.append(run(b, device, workspace=ws)), need)
+    assert split != whole
+    check(got[0], reference(b), dtype)
