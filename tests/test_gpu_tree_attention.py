@@ -356,3 +356,24 @@ def test_units_whole_or_in_pieces(device, code, dtype, n, longest, whole):
     split = pieces_written(lambda ws: got.append(run(b, device, workspace=ws)), need)
     assert split != whole
     check(got[0], reference(b), dtype)
+
+
+@pytest.mark.parametrize("code", [None] + CODES)
+@pytest.mark.parametrize("bad", [1 << 30, -2])
+def test_rows_of_block_ids_outside_the_cache(device, code, bad):
+    """Such an id reads block 0, in every row that sees its keys, and nothing else
+    changes."""
+    _say(f"tree bad ids {code} {bad}")
+    b = make_trees(37, device, (4, 2, 64), [40, 3, 2000], [10, 70, 5], torch.bfloat16, code,
+                   fill=0.0)
+    at = ((0, 1), (1, 4), (2, 60))                # committed and drafted keys
+    want = dict(b, tables=b["tables"].clone())
+    for i, j in at:
+        assert j * BS < int(b["ctx"][i])
+        want["tables"][i, j] = 0
+        b["tables"][i, j] = bad
+    ops.device_errors()
+    got = run(b, device)
+    assert ops.device_errors() == _hip.LV_DEVERR_BLOCK_ID
+    check(got, reference(want), torch.bfloat16)
+    assert ops.device_errors() == 0
