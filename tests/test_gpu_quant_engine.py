@@ -229,3 +229,52 @@ def test_native_and_python_paths_agree(device, monkeypatch):
     monkeypatch.setattr(ops, "_native_module", none)
     for x, y in zip(native, calls()):
         assert torch.equal(x, y)
+
+
+def test_native_calls_serve_plain_arguments(device, monkeypatch):
+    """Each wrapper's native call takes the arguments of a serving step itself: it
+    returns a result, not None, which hands the call to the Python path."""
+    _say("native calls")
+    from test_gpu_quant_cache import make_batch
+    from test_gpu_tree_attention import make_trees
+    b = make_batch(41, device, (8, 2, 64), [300, 40, 90], [1, 1, 30], torch.bfloat16, torch.int8)
+    t = make_trees(42, device, (8, 2, 64), [100, 9], [12, 40], torch.bfloat16)
+    c = make_trees(43, device, (8, 2, 64), [100, 9], [12, 40], torch.float16, torch.float8_e4m3fn)
+    b, t, c = ({k: v.to(device) if torch.is_tensor(v) else v for k, v in x.items()}
+               for x in (b, t, c))
+    # the stream's scratch buffer, which only the Python path makes
+    ops._workspace(torch.device("cuda", torch.cuda.current_device()), 64 << 20)
+    native, seen = ops._native_module or ops._native(), []
+    names = ("kv_scatter_quant", "kv_gather_quant", "qk_norm_rope_cache_quant",
+             "paged_attention_quant", "tree_attention", "tree_attention_quant")
+
+    def watched(name):
+        def call(*args):
+            result = getattr(native, name)(*args)
+            seen.append((name, result is not None))
+            return result
+        return call
+    monkeypatch.setattr(ops, "_native_module",
+                        types.SimpleNamespace(**{n: watched(n) for n in names}))
+    slots = torch.arange(9, device=device)
+    for code in (torch.int8, torch.float8_e4m3fn):
+        for dtype in (torch.bfloat16, torch.float16, torch.float32):
+            cache = ops.quant_kv_cache(4, 16, 2, 64, code, device)
+            qkv = torch.ones(9, 12 * 64, dtype=dtype, device=device)
+            x = qkv.view(9, 12, 64)
+            cos = torch.ones(50, 32, dtype=dtype, device=device)
+            ops.kv_scatter_quant(x[:, 8:10], x[:, 10:], cache, slots)
+            ops.kv_gather_quant(cache, slots, dtype)
+            ops.qk_norm_rope_cache_quant(qkv, 8, 2, 64, cos, cos, slots, slots, cache)
+            ops.qk_norm_rope_cache_quant(qkv, 8, 2, 64, cos, cos, slots, slots, cache,
+                                         q_norm_weight=cos.view(-1)[:64],
+                                         k_norm_weight=cos.view(-1)[:64], eps=1e-5)
+    for decodes, kw in ((2, {}), (0, dict(out=torch.empty_like(b["q"])))):
+        ops.paged_attention_quant(b["q"], b["cache"], b["tables"], b["ctx"], scale=0.1,
+                                  cu_seqlens=b["cu"], num_decodes=decodes, max_query_len=30, **kw)
+    ops.paged_attention_quant(b["q"][:3], b["cache"], b["tables"], b["ctx"], scale=0.1)
+    for y, op, kv in ((t, ops.tree_attention, t.get("kv")),
+                      (c, ops.tree_attention_quant, [c.get("cache")])):
+        op(y["q"], *kv, y["tables"], y["ctx"], y["cu"], y["mask"], scale=0.1, max_query_len=40)
+    assert set(n for n, _ in seen) == set(names)
+    assert all(served for _, served in seen), [n for n, served in seen if not served]
