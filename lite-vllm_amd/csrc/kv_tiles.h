@@ -407,11 +407,13 @@ void attn_tile_kernel(TileArgs a) {
   constexpr int OPC = E::kPer16B < 8 ? 1 : E::kPer16B / 8;             // operand chunks of a cached chunk
   constexpr bool kWide = P::kWide;
   static_assert(16 % RPL == 0, "whole loads per block");
-  // K and V tile, then the scales of its keys; the merge of a piece's parts
-  // reuses the tiles (4 wavefronts x 32 rows x D floats at most)
+  // K and V tiles, then the scales of their keys; the merge of a piece's parts
+  // reuses the tiles (WAVES x 32 rows x D floats, which fill them for eight
+  // wavefronts)
   extern __shared__ __align__(16) unsigned char s_dyn[];
   // (of K or V, in 16-bit places)
   constexpr int NST = F::NST, TILE = KT * D * (kWide ? 2 : 1);
+  static_assert(KW == 1 || F::WAVES * 32 * D * 4 <= NST * 2 * TILE * 2, "the merge fits the tiles");
   uint16_t* const s_kv = reinterpret_cast<uint16_t*>(s_dyn);       // [NST][K, V][TILE]
   // [NST][KT] each: K's scales; V's scales, or their logarithms and inverses
   float* const s_sc = reinterpret_cast<float*>(s_kv + NST * 2 * TILE);
