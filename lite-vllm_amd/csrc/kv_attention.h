@@ -91,6 +91,7 @@ struct TilePlan {
   int seq_begin, n_seqs, max_q;
   int rw;                   // tile kernel: 32-row groups of a unit, 1, 2, 4 or 8; 0: narrow kernel
   int waves;                // and its wavefronts
+  int64_t list;             // tiles of all units, at most
   int grid, ranges;         // workgroups; ranges that the list is split into
   int direct, nq;           // (see TileArgs)
   int slot_heads, slot_rows;

@@ -112,8 +112,9 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   const int64_t units = units_of(r);
   const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_blocks * kBs + kt - 1) / kt);
   p.nq = (int)((rows + r - 1) / r);
+  p.list = units * tiles;
   const int64_t at_once = cus * (f32 || p.waves == 8 ? 1 : 2);
-  p.ranges = (int)std::min<int64_t>(units * tiles, at_once);
+  p.ranges = (int)std::min<int64_t>(p.list, at_once);
   p.grid = p.ranges;
   const bool one_round = units <= at_once;
   const int64_t all = (groups + kXcds - 1) / kXcds * kXcds * p.nq;
@@ -136,9 +137,8 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
     p.direct = 0;
     p.slot_heads = std::min(num_kv_heads, 8);
     while (num_kv_heads % p.slot_heads != 0) --p.slot_heads;
-    const int64_t list = (int64_t)n_seqs * (num_kv_heads / p.slot_heads) *
-                         std::max(1, (max_blocks + 1) / 2);
-    p.grid = p.ranges = (int)std::min<int64_t>(list, cus * (8 / p.slot_heads));
+    p.list = (int64_t)n_seqs * (num_kv_heads / p.slot_heads) * std::max(1, (max_blocks + 1) / 2);
+    p.grid = p.ranges = (int)std::min<int64_t>(p.list, cus * (8 / p.slot_heads));
   }
   if (p.direct < 2) {
     const size_t slots = (size_t)2 * p.ranges * p.slot_heads * p.slot_rows;
@@ -231,15 +231,18 @@ int check_call(const char* who, Call& a, int num_decodes, const void* query, int
   a.r.num_heads = num_heads; a.r.num_kv_heads = num_kv_heads;
   a.r.scale_log2 = scale * 1.4426950408889634f;
   a.d = head_dim; a.dtype = dtype;
-  const int64_t g = num_heads / num_kv_heads;
-  const int64_t units = (int64_t)num_seqs * num_kv_heads * ((max_query_len * g + 31) / 32);
-  LV_REQUIRE(units * std::max(1, max_blocks / 4 + 1) < (1ll << 31) - (1 << 16) &&
-                 max_query_len * g < (1ll << 30),
-             "%s: too many keys and rows for 32-bit offsets", who);
   if (num_seqs > 16384) {
     set_error("%s: %d sequences (up to 16384 are supported)", who, num_seqs);
     return LV_ERR_UNSUPPORTED;
   }
+  bool fits = max_query_len * (int64_t)(num_heads / num_kv_heads) < (1ll << 30);
+  for (const bool codes : {false, true})
+    for_each_part(num_seqs, num_decodes, max_query_len, num_heads, num_kv_heads, head_dim,
+                  max_blocks, dtype, codes, [&](const TilePlan& p) {
+                    fits = fits && p.list < (1ll << 31) - (1 << 16);
+                    return LV_OK;
+                  });
+  LV_REQUIRE(fits, "%s: too many keys and rows for 32-bit offsets", who);
   const size_t need = workspace_size(num_seqs, num_decodes, max_query_len, num_heads, num_kv_heads,
                                      head_dim, max_blocks, dtype);
   if (need > 0 && (!ws || ((uintptr_t)ws & 255) != 0 || ws_bytes < need)) {

@@ -82,6 +82,23 @@ def test_attention_refusals():
     assert attend(B=0, T=0) == 0 and attend(T=0) == 0          # nothing to do
 
 
+def test_places_of_the_list_fit_32_bits():
+    """A launch's tiles are counted in 32 bits, so as many as its own sequences can
+    have are refused past them; those of the call's other launches do not count.
+    (No workspace: what is accepted ends there.)"""
+    wide = cache(num_kv_heads=8, stride_block=8 * 16 * 64, scale_stride_block=8 * 16)
+    # one long chunk beside decode rows
+    refused(attend(c=wide, qs=4096, os=4096, H=64, mb=8192, B=256, nd=255, T=255 + 8192, mq=8192,
+                   wsb=0), "workspace", -3)
+    # chunks alone, and decode rows of up to 8 heads a kv head, in tiles of 32 keys
+    refused(attend(c=wide, qs=4096, os=4096, H=64, mb=1 << 20, B=256, T=256 * 8192, mq=8192,
+                   wsb=0), "32-bit offsets")
+    one = cache(num_kv_heads=1, stride_block=16 * 64, scale_stride_block=16)
+    many = dict(c=one, qs=64, os=64, H=1, B=4096, nd=4096, T=4096, mq=1, wsb=0)
+    refused(attend(mb=1 << 20, **many), "32-bit offsets")
+    refused(attend(mb=1 << 19, **many), "workspace", -3)
+
+
 def test_tree_refusals():
     lib = _hip.load()
 
