@@ -89,14 +89,14 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   // stays with long rows: few units, or long contexts of codes, whose way into
   // LDS they share.  Where there are many short units two workgroups hide each
   // other's starts.  us with eight | four: 48 trees of 40-64 tokens at 500-4000
-  // 134 | 139, of 12-16 tokens 99 | 114, 4 trees over codes 37.5 | 45, two
-  // chunks of 700-1024 at 15000-19000 292 | 343, 60 chunks of 100 at 0-3000
-  // 140 | 159; 256 trees of 40-64 at 300-1000 323 | 228, at 1000-3000 627 | 533,
-  // 60 chunks of 100 at 0-300 54 | 47.  33-64 rows on four wavefronts are half
+  // 136 | 142, of 12-16 tokens 100 | 114, 4 over codes at 2000-16000 39 | 50, two
+  // chunks of 700-1024 at 15000-19000 372 | 413, 60 chunks of 100 at 0-3000
+  // 170 | 188; 256 trees of 40-64 at 300-1000 317 | 224, at 1000-3000 616 | 537,
+  // 60 chunks of 100 at 0-300 60 | 51.  33-64 rows on four wavefronts are half
   // a unit of RW = 4, since RW = 2 on four has too few registers (48 trees of
   // 20-32 tokens at 500-4000 173, RW = 4 125, RW = 2 on eight 102).  Up to 32
-  // rows over codes stay with four (16 trees of 4-8 tokens at 2000-16000 90 |
-  // 67).  fp32 keeps to four: its registers and LDS are those of one wavefront a
+  // rows over codes stay with four (16 trees of 4-8 tokens at 2000-16000 98 |
+  // 72).  fp32 keeps to four: its registers and LDS are those of one wavefront a
   // SIMD.
   if (!f32) {
     const int wide = std::max(p.rw, 2);
@@ -121,10 +121,10 @@ TilePlan plan_tiles(int seq_begin, int n_seqs, int max_q, int num_heads, int num
   if (all < (1ll << 31)) {
     // Contexts of a few tiles are not split where all units run at once (a join
     // takes as long as two tiles or three: 3 decode rows of 40-300 keys 7.9 us,
-    // split 10.6, through the narrow kernel 10.6; up to 8 tiles a tree of 700
+    // split, by the narrow kernel, 10.4, and 11.0 where the table is wide; up to 8 tiles a tree of 700
     // keys takes 15.0, split 13.4).  Where there are half as many units again as
     // run at once, the kernel looks whether they need to be (15 chunks of 512
-    // at 0-3071 beside decode rows 317 us, split 393).
+    // at 0-3071 203 us, split 265).
     p.direct = one_round && tiles <= 4 ? 3 : tiles <= 2 ? 2 : 2 * units >= 3 * p.ranges ? 1 : 0;
     if (p.direct) p.grid = (int)std::max<int64_t>(all, p.direct == 1 ? p.ranges : 0);
   }

@@ -23,7 +23,7 @@ namespace lv {
 // workgroup takes a whole unit instead (direct), longest sequences and last
 // rows first, so that there are no pieces: 15 chunks of 512 tokens at offsets
 // of 0-3071, 2 query heads for each of 8 kv heads (480 units of 256 rows),
-// beside 192 decode rows 393 -> 317 us.
+// 265 -> 203 us.
 //
 // A workgroup is 4 or 8 wavefronts: RW groups of 32 rows times KW = WAVES / RW
 // parts of every tile's keys, so that few rows (RW = 1: decodes, small trees)
@@ -43,7 +43,8 @@ namespace lv {
 // 16 keys, and by DPP into the instruction that takes them: read as they lie
 // for 16 keys (b128, the same for 32 lanes) they were most of the LDS time (two
 // chunks of 700-1024 tokens at 15000-19000, 8 query heads a kv head, 309 -> 292
-// us; trees of 25-60 tokens at 2000-16000 213 -> 198).
+// us; trees of 25-60 tokens at 2000-16000 213 -> 198; both with weights of one
+// part).
 //
 // Weights.  A weight rounded to bf16 (2^-8) or, for an fp16 output, to fp16
 // (2^-11) errs as much as the output's own rounding does, and the keys' errors
@@ -68,10 +69,11 @@ namespace lv {
 // TFLOP/s at most; six products of bf16 parts would need three times the LDS):
 // trees of 40-64 tokens at 500-4000, 48 sequences, 8 kv heads of 128: 594 us.
 //
-// What bounds it: over a 16-bit cache HBM, 131 us for those trees in bf16
-// (3.6 TB/s); the chunks above at 377 us the issue of one SIMD's two wavefronts
-// (registers allow no third), whose products (40% of the time) and vector
-// instructions (65%) overlap little.
+// What bounds it: the chunks above, at 373 us, the issue of one SIMD's two
+// wavefronts (registers allow no third), whose products (46% of the cycles) and
+// vector instructions (52%) overlap little.  Over a 16-bit cache the one tile that
+// is on its way from HBM while another is computed: those trees in bf16 take 132 us,
+// 3.6 TB/s, with products 29% and vector instructions 36% of the cycles.
 //
 // Zero weights times a value that is not finite make NaN: a piece whose sums
 // are not finite is computed again key by key (careful), where a key that a
@@ -1003,7 +1005,8 @@ void attn_tile_kernel(TileArgs a) {
       for (int i = t, st = 0; i < t1; ++i, st ^= 1) {
         // Of eight wavefronts the second four, which share the SIMDs of the
         // first, write half a tile later: one multiplies while the other does
-        // not (214 -> 202 us for trees of 64 tokens, 8 query heads a kv head).
+        // not (214 -> 202 us for trees of 25-60 tokens over codes, with weights of
+        // one part).
 #pragma unroll 1
         for (int sub = 0; sub < F::SUB; ++sub) {
           if (i + 1 < t1 && sub == (F::SUB == 2 ? wave >> 2 : 0)) {
